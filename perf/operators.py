@@ -323,7 +323,8 @@ def work(case):
 # ------------------------------------------------------------------------------------------- in 64 bits
 def _e4m3_nearest(x):
     """x rounded to the e4m3 grid: 4 significant bits, exponents from -6, ties to even, at most 448."""
-    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -20))).clamp(min=-6) - 3)
+    _, e = torch.frexp(x.abs())                      # x in [2^(e - 1), 2^e); a rounded logarithm would miss powers of two
+    step = torch.exp2((e.double() - 1).clamp(min=-6) - 3)
     return (torch.round(x / step) * step).clamp(-448, 448)
 
 
@@ -351,7 +352,10 @@ def _cache_exact(s):
         if c["cache"] == "e4m3":
             power = torch.exp2(b.flatten(0, 1).double() - 127)
             top = x.abs().amax(-1)
-            e = torch.where(top > 0, torch.ceil(torch.log2(top / 448)), torch.zeros_like(top)).clamp(-126, 127)
+            e = torch.zeros_like(top)
+            for k in range(-126, 128):                  # the smallest integer e with top <= 448 * 2^e
+                e += (top > 448 * 2.0 ** (k - 1)) & (top > 0)
+            e = torch.where(top > 0, e - 127, e).clamp(min=-126)
             held = held * power[..., None]
             held[s["write_slots"]] = _e4m3_nearest(x / torch.exp2(e)[..., None]) * torch.exp2(e)[..., None]
             b = b.clone()
