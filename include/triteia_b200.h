@@ -221,6 +221,66 @@ int trb_rotary_embedding(const void* positions, void* query, void* key, const vo
                          long long key_stride, int num_heads, int num_kv_heads, int head_size,
                          int is_neox, int dtype, int dev, void* stream);
 
+/* Root-mean-square norm of every query and key head and the position rotation, in one pass: y = x / sqrt(mean x^2 +
+ * eps) * weight over each head, then the first rot_dim elements of y rotated as trb_rotary_embedding does, 32-bit
+ * arithmetic and one rounding.  query [T, num_heads * head_size] and key [T, num_kv_heads * head_size] (NULL with
+ * num_kv_heads 0) have rows `*_stride` elements apart (multiples of 8, 16-byte aligned: parts of a fused q/k/v
+ * product); query_out / key_out likewise, and may be the inputs.  Weights [head_size] of `dtype`, NULL: ones.
+ * cos_sin_cache [max_position, rot_dim] of `dtype`, or of 32-bit floats with cache_is_f32; positions int64 [T]; a token
+ * whose position is outside [0, max_position) is left alone (its output rows are not written).
+ * head_size % 8 == 0, at most 256.  The reference has the rotation alone (csrc/ops/pos_encoding_kernels.cu:118-160). */
+int trb_qk_norm_rotary(const void* positions, const void* query, void* query_out, const void* key, void* key_out,
+                       const void* query_weight, const void* key_weight, const void* cos_sin_cache, int cache_is_f32,
+                       long long max_position, int num_tokens, int rot_dim, long long query_stride,
+                       long long query_out_stride, long long key_stride, long long key_out_stride, int num_heads,
+                       int num_kv_heads, int head_size, float eps, int is_neox, int dtype, int dev, void* stream);
+
+/* Keys and values of T tokens into a paged cache, and tokens read back.  The cache's element [page, place, head, d] lies
+ * at page * page_stride + place * token_stride + head * head_stride + d, the same for keys and values (strides in
+ * elements, multiples of 8); slots int64 [T], slot = page * page_size + place.  Exponents NULL: the cache holds `dtype`.
+ * Else it holds e4m3 codes and for every (token, head) an exponent byte b (strides exp_*), value = code * 2^(b - 127):
+ * b - 127 is the smallest integer e with max |x| <= 448 * 2^e over the finite values of the head (0 for a head of zeros,
+ * never below -126), codes are rounded to nearest even, infinities and NaN become NaN.
+ *   trb_cache_write  a token whose slot is outside [0, num_pages * page_size) is skipped (padding); each slot at most
+ *                    once in a call (of two tokens with one slot, parts of either may be stored)
+ *   trb_cache_read   key_out / value_out [T, heads, head_size] contiguous of `dtype`; zeros for a slot outside the cache
+ * head_size % 8 == 0, at most 256; inputs' strides multiples of 8, 16-byte aligned (e4m3 caches: 8-byte aligned).
+ * No counterpart in the reference: its attention files take a cache that the serving engine fills
+ * (triteia/triton/decode_attention.py:30-120). */
+int trb_cache_write(const void* key, const void* value, const void* slots, void* key_cache, void* value_cache,
+                    void* key_exponents, void* value_exponents, int num_tokens, int heads, int head_size, int page_size,
+                    long long num_pages, long long key_token_stride, long long key_head_stride,
+                    long long value_token_stride, long long value_head_stride, long long page_stride,
+                    long long token_stride, long long head_stride, long long exp_page_stride, long long exp_token_stride,
+                    long long exp_head_stride, int dtype, int dev, void* stream);
+int trb_cache_read(const void* key_cache, const void* value_cache, const void* key_exponents, const void* value_exponents,
+                   const void* slots, void* key_out, void* value_out, int num_tokens, int heads, int head_size,
+                   int page_size, long long num_pages, long long page_stride, long long token_stride,
+                   long long head_stride, long long exp_page_stride, long long exp_token_stride, long long exp_head_stride,
+                   int dtype, int dev, void* stream);
+
+/* Attention of new tokens over a paged cache (as above; token and head strides times the element size multiples of 16
+ * bytes).  Sequence b has lengths[b] tokens in the cache (int32), its j-th on page page_table[b, j / page_size] (int32,
+ * rows table_stride apart, table_width entries; only entries below lengths[b] / page_size rounded up are read).  Its new
+ * tokens are rows [query_starts[b], query_starts[b + 1]) of query (int32 [num_seqs + 1]; NULL: one token per sequence,
+ * num_tokens == num_seqs) and are the last ones of the lengths[b].  Token i of n stands at p = lengths[b] - n + i and
+ * sees the keys j < lengths[b] with j <= p (causal) and j > p - window (window > 0, causal only):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j, zero where nothing is seen; query head h reads key head
+ *   h / (num_heads / num_kv_heads).
+ * A page outside [0, num_pages) counts as masked; a length beyond table_width * page_size counts as that.  Rows of out
+ * outside every sequence are not written.  What lies in the cache at or beyond a sequence's length is never used; keys and
+ * values below it are expected to be finite numbers.
+ * query and out [T, num_heads, head_size] of `dtype` with strides that are multiples of 8; head_size 64 or 128.
+ * Stands for the programs of triteia/triton/decode_attention.py:30-214 and extend_attention.py:39-170. */
+int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
+                        const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,
+                        void* out, int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                        int page_size, long long num_pages, long long table_stride, int table_width,
+                        long long query_token_stride, long long query_head_stride, long long out_token_stride,
+                        long long out_head_stride, long long page_stride, long long token_stride, long long head_stride,
+                        long long exp_page_stride, long long exp_token_stride, long long exp_head_stride, float scale,
+                        int causal, int window, int dtype, int dev, void* stream);
+
 /* sums[r] = (accumulate ? sums[r] : 0) + sum over n of y[r, n]: fp32 per-row checksum of an fp16
  * matrix [rows, prob_m] (prob_m % 8 == 0, y 16-byte aligned), fixed summation order.  Used by the
  * sharded linear-stack scenario (a full Llama-2-7B-shaped stack of independent delta linears) to return

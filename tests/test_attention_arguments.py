@@ -1,0 +1,127 @@
+"""Calls that the cache, norm-and-rotation and attention operators refuse before anything reaches the device (no GPU: on a
+CPU tensor the refusal of the device comes last or first, never a launch)."""
+import ctypes
+
+import pytest
+import torch
+
+from triteia_b200 import _lib, capi, ops
+
+H, D, P, PAGES = 2, 64, 16, 4
+
+
+def test_cpu_tensors_are_rejected():
+    kc, vc, _, _ = ops.new_cache(PAGES, P, H, D, device="cpu")
+    x, slots = torch.zeros(3, H, D, dtype=torch.float16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.cache_write(x, x, kc, vc, slots)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.cache_read(kc, vc, slots)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_attention(x, kc, vc, torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        capi.qk_norm_rotary_embedding(slots, x.view(3, -1), x.view(3, -1), D, torch.zeros(8, D, dtype=torch.float16), True)
+
+
+def _attention(**change):
+    """trb_paged_attention with a good set of arguments but for `change`; the pointers are never read: every call that is
+    made here is refused on the host."""
+    a = dict(query=64, key_cache=64, value_cache=64, key_exponents=None, value_exponents=None, page_table=64, lengths=64, query_starts=64,
+             out=64, num_tokens=3, num_seqs=2, num_heads=4, num_kv_heads=2, head_size=64, page_size=16, num_pages=4, table_stride=2,
+             table_width=2, query_token_stride=256, query_head_stride=64, out_token_stride=256, out_head_stride=64, page_stride=2048,
+             token_stride=128, head_stride=64, exp_page_stride=0, exp_token_stride=0, exp_head_stride=0, scale=0.125, causal=1, window=0,
+             dtype=0, dev=0, stream=None)
+    assert set(change) <= set(a)
+    return _lib.lib.trb_paged_attention(*{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(query=None), 3), (dict(key_cache=None), 3), (dict(value_cache=None), 3), (dict(lengths=None), 3), (dict(out=None), 3),
+    (dict(page_table=None), 3), (dict(key_exponents=64), 3), (dict(value_exponents=64), 3), (dict(num_tokens=-1), 3),
+    (dict(num_seqs=-1), 3), (dict(num_heads=0), 3), (dict(num_kv_heads=0), 3), (dict(page_size=0), 3), (dict(num_pages=-1), 3),
+    (dict(table_width=-1), 3), (dict(window=-1), 3), (dict(query_starts=None), 3),
+    (dict(num_heads=5), 1), (dict(window=4, causal=0), 1), (dict(query=72), 1), (dict(out=72), 1), (dict(key_cache=72), 1),
+    (dict(value_cache=66), 1), (dict(query_token_stride=257), 1), (dict(out_head_stride=66), 1), (dict(token_stride=132), 1),
+    (dict(table_width=1 << 28, page_size=64), 1), (dict(num_tokens=1 << 30, num_heads=8), 1),
+    (dict(head_size=80), 2), (dict(head_size=256), 2), (dict(dtype=2), 2),
+])
+def test_attention_refuses_on_the_host(change, code):
+    assert _attention(**change) == code
+
+
+def test_attention_without_tokens_or_sequences_does_nothing():
+    assert _attention(num_tokens=0) == 0
+    assert _attention(num_seqs=0) == 0
+
+
+def _write(**change):
+    a = dict(key=64, value=64, slots=64, key_cache=64, value_cache=64, key_exponents=None, value_exponents=None, num_tokens=3, heads=2,
+             head_size=64, page_size=16, num_pages=4, key_token_stride=128, key_head_stride=64, value_token_stride=128,
+             value_head_stride=64, page_stride=2048, token_stride=128, head_stride=64, exp_page_stride=0, exp_token_stride=0,
+             exp_head_stride=0, dtype=0, dev=0, stream=None)
+    return _lib.lib.trb_cache_write(*{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(key=None), 3), (dict(value=None), 3), (dict(slots=None), 3), (dict(key_cache=None), 3), (dict(value_cache=None), 3),
+    (dict(key_exponents=64), 3), (dict(num_tokens=-1), 3), (dict(heads=0), 3), (dict(page_size=0), 3), (dict(num_pages=-1), 3),
+    (dict(head_size=60), 1), (dict(head_size=264), 1), (dict(key=72), 1), (dict(value_cache=72), 1), (dict(key_token_stride=132), 1),
+    (dict(value_head_stride=65), 1), (dict(head_stride=68), 1), (dict(dtype=5), 2),
+])
+def test_cache_write_refuses_on_the_host(change, code):
+    assert _write(**change) == code
+
+
+def _norm(**change):
+    a = dict(positions=64, query=64, query_out=64, key=64, key_out=64, query_weight=64, key_weight=64, table=64, cache_is_f32=0,
+             max_position=8, num_tokens=3, rot_dim=64, query_stride=128, query_out_stride=128, key_stride=64, key_out_stride=64,
+             num_heads=2, num_kv_heads=1, head_size=64, eps=1e-6, is_neox=1, dtype=0, dev=0, stream=None)
+    return _lib.lib.trb_qk_norm_rotary(*{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(positions=None), 3), (dict(query=None), 3), (dict(query_out=None), 3), (dict(key=None), 3), (dict(key_out=None), 3),
+    (dict(table=None), 3), (dict(num_tokens=-1), 3), (dict(num_heads=0), 3), (dict(num_kv_heads=-1), 3), (dict(max_position=-1), 3),
+    (dict(head_size=60, rot_dim=60), 1), (dict(head_size=264), 1), (dict(rot_dim=63), 1), (dict(rot_dim=66), 1), (dict(query=72), 1),
+    (dict(key_out=72), 1), (dict(query_stride=132), 1), (dict(key_stride=65), 1), (dict(dtype=3), 2),
+])
+def test_norm_and_rotation_refuse_on_the_host(change, code):
+    assert _norm(**change) == code
+
+
+def test_norm_and_rotation_of_no_tokens_do_nothing():
+    assert _norm(num_tokens=0) == 0
+
+
+def _cache(quantised=False):
+    return ops.new_cache(PAGES, P, H, D, device="cpu", quantised=quantised)
+
+
+@pytest.mark.parametrize("spoil,what", [
+    (lambda c: (c[0], c[1][:-1], c[2], c[3]), "same strides"),
+    (lambda c: (c[0], c[1].transpose(1, 2).contiguous().transpose(1, 2), c[2], c[3]), "same strides"),
+    (lambda c: (c[0].to(torch.float32), c[1].to(torch.float32), c[2], c[3]), "the cache holds"),
+    (lambda c: (c[0], c[1], torch.zeros(PAGES, P, H, dtype=torch.uint8), None), "the cache holds|go together"),
+    (lambda c: (c[0][..., ::2], c[1][..., ::2], c[2], c[3]), "contiguous last dimension"),
+    (lambda c: (c[0][:, :0], c[1][:, :0], c[2], c[3]), "page size"),
+])
+def test_caches_that_do_not_fit_are_refused(spoil, what):
+    from triteia_b200.ops.attention.kv_cache import check_cache
+
+    with pytest.raises(RuntimeError, match=what):
+        check_cache(*spoil(_cache()), torch.float16, torch.device("cpu"))
+
+
+@pytest.mark.parametrize("spoil,what", [
+    (lambda c: (c[0], c[1], c[2], None), "go together"),
+    (lambda c: (c[0], c[1], None, None), "the cache holds"),
+    (lambda c: (c[0], c[1], c[2].int(), c[3].int()), "uint8"),
+    (lambda c: (c[0], c[1], c[2][:1], c[3][:1]), "uint8"),
+    (lambda c: (c[0], c[1], c[2], c[3].transpose(0, 1).contiguous().transpose(0, 1)), "same strides"),
+])
+def test_quantised_caches_that_do_not_fit_are_refused(spoil, what):
+    from triteia_b200.ops.attention.kv_cache import check_cache
+
+    assert check_cache(*_cache(True), torch.bfloat16, torch.device("cpu"))[:4] == (PAGES, P, H, D)
+    with pytest.raises(RuntimeError, match=what):
+        check_cache(*spoil(_cache(True)), torch.float16, torch.device("cpu"))

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_PKG, "libtriteia_b200.so")
 TRB_OK, ERR_PROB_SHAPE, ERR_KERN_SHAPE, ERR_BAD_ARG, ERR_CUDA, ERR_TIMEOUT, ERR_SCRATCH = range(7)
 TRB_F16, TRB_BF16 = 0, 1
 
-_vp, _i, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 
 # name -> (restype, argtypes); must list every function of include/triteia_b200.h
 SIGNATURES = {
@@ -44,6 +44,10 @@ SIGNATURES = {
     "trb_gelu_quick": (_i, [_vp, _vp, ctypes.c_longlong, _i, _i, _vp]),
     "trb_silu_and_mul": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "trb_rotary_embedding": (_i, [_vp] * 5 + [_i, _i, ctypes.c_longlong, ctypes.c_longlong] + [_i] * 6 + [_vp]),
+    "trb_qk_norm_rotary": (_i, [_vp] * 8 + [_i, _ll, _i, _i] + [_ll] * 4 + [_i] * 3 + [_f, _i, _i, _i, _vp]),
+    "trb_cache_write": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 11 + [_i, _i, _vp]),
+    "trb_cache_read": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 7 + [_i, _i, _vp]),
+    "trb_paged_attention": (_i, [_vp] * 9 + [_i] * 6 + [_ll, _ll, _i] + [_ll] * 10 + [_f] + [_i] * 4 + [_vp]),
     "trb_row_checksum": (_i, [_vp] * 2 + [_i] * 4 + [_vp]),
     "trb_stack_scratch_bytes": (_sz, [_i, _i]),
     "trb_stack_pass": (_i, [_i] + [_vp] * 5 + [_i, _vp] + [_vp] * 5 + [_i, _i, _vp, _i, _vp, _sz, _i, _vp]),

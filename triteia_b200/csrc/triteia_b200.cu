@@ -16,4 +16,7 @@
 #include "lora.cuh"
 #include "base_gemm.cuh"
 #include "elementwise.cuh"
+#include "qk_norm.cuh"
+#include "kv_cache.cuh"
+#include "attention.cuh"
 #include "no_alloc.cuh"
