@@ -1,7 +1,5 @@
-"""Calls that the cache, norm-and-rotation and attention operators refuse before anything reaches the device (no GPU: on a
-CPU tensor the refusal of the device comes last or first, never a launch)."""
-import ctypes
-
+"""Calls that the cache, norm-and-rotation and attention operators refuse before anything reaches the device (no GPU: the
+check for a CUDA device comes last)."""
 import pytest
 import torch
 
@@ -97,22 +95,30 @@ def _cache(quantised=False):
     return ops.new_cache(PAGES, P, H, D, device="cpu", quantised=quantised)
 
 
+SLOTS = torch.zeros(3, dtype=torch.int64)
+
+
 @pytest.mark.parametrize("spoil,what", [
     (lambda c: (c[0], c[1][:-1], c[2], c[3]), "same strides"),
     (lambda c: (c[0], c[1].transpose(1, 2).contiguous().transpose(1, 2), c[2], c[3]), "same strides"),
     (lambda c: (c[0].to(torch.float32), c[1].to(torch.float32), c[2], c[3]), "the cache holds"),
-    (lambda c: (c[0], c[1], torch.zeros(PAGES, P, H, dtype=torch.uint8), None), "the cache holds|go together"),
+    (lambda c: (c[0], c[1], torch.zeros(PAGES, P, H, dtype=torch.uint8), None), "go together"),
     (lambda c: (c[0][..., ::2], c[1][..., ::2], c[2], c[3]), "contiguous last dimension"),
     (lambda c: (c[0][:, :0], c[1][:, :0], c[2], c[3]), "page size"),
+    (lambda c: (c[0][0], c[1][0], c[2], c[3]), "same strides"),
 ])
 def test_caches_that_do_not_fit_are_refused(spoil, what):
-    from triteia_b200.ops.attention.kv_cache import check_cache
-
-    with pytest.raises(RuntimeError, match=what):
-        check_cache(*spoil(_cache()), torch.float16, torch.device("cpu"))
+    kc, vc, ke, ve = spoil(_cache())
+    x = torch.zeros(3, H, D, dtype=torch.float16)
+    for call in (lambda: ops.cache_write(x, x, kc, vc, SLOTS, ke, ve), lambda: ops.cache_read(kc, vc, SLOTS, ke, ve, dtype=torch.float16),
+                 lambda: ops.paged_attention(x, kc, vc, torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32), key_exponents=ke,
+                                             value_exponents=ve)):
+        with pytest.raises(RuntimeError, match=what):
+            call()
 
 
 @pytest.mark.parametrize("spoil,what", [
+    (lambda c: c, "CUDA"),
     (lambda c: (c[0], c[1], c[2], None), "go together"),
     (lambda c: (c[0], c[1], None, None), "the cache holds"),
     (lambda c: (c[0], c[1], c[2].int(), c[3].int()), "uint8"),
@@ -120,8 +126,66 @@ def test_caches_that_do_not_fit_are_refused(spoil, what):
     (lambda c: (c[0], c[1], c[2], c[3].transpose(0, 1).contiguous().transpose(0, 1)), "same strides"),
 ])
 def test_quantised_caches_that_do_not_fit_are_refused(spoil, what):
-    from triteia_b200.ops.attention.kv_cache import check_cache
-
-    assert check_cache(*_cache(True), torch.bfloat16, torch.device("cpu"))[:4] == (PAGES, P, H, D)
+    kc, vc, ke, ve = spoil(_cache(True))
+    x = torch.zeros(3, H, D, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match=what):
-        check_cache(*spoil(_cache(True)), torch.float16, torch.device("cpu"))
+        ops.cache_write(x, x, kc, vc, SLOTS, ke, ve)
+    with pytest.raises(RuntimeError, match=what):
+        ops.cache_read(kc, vc, SLOTS, ke, ve, dtype=torch.bfloat16)
+
+
+def _attend(**change):
+    kc, vc, _, _ = _cache()
+    a = dict(query=torch.zeros(3, 4, D, dtype=torch.float16), key_cache=kc, value_cache=vc, page_table=torch.zeros(3, 2, dtype=torch.int32),
+             lengths=torch.ones(3, dtype=torch.int32)) | change
+    return ops.paged_attention(**a)
+
+
+Q = torch.zeros(3, 4, D, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(), "CUDA"), (dict(lengths=torch.ones(3, dtype=torch.int64)), "lengths"), (dict(lengths=torch.ones(2, dtype=torch.int32)), "lengths"),
+    (dict(query_starts=torch.ones(3, dtype=torch.int32)), "query_starts"), (dict(query_starts=torch.ones(8, dtype=torch.int32)[::2]), "query_starts"),
+    (dict(page_table=torch.zeros(3, 2, dtype=torch.int64)), "page_table"), (dict(page_table=torch.zeros(3, 4, dtype=torch.int32)[:, ::2]), "page_table"),
+    (dict(page_table=torch.zeros(2, 2, dtype=torch.int32), lengths=torch.ones(2, dtype=torch.int32)), "query_starts is needed"),
+    (dict(window=0), "window"), (dict(window=-3), "window"), (dict(window=3, causal=False), "window"), (dict(query=Q[:, :3]), "do not go with"),
+    (dict(query=Q[:, :0]), "do not go with"), (dict(query=Q[..., :32]), "do not go with"), (dict(query=Q.bfloat16()), "the cache holds"),
+    (dict(query=Q[0]), "query must be"), (dict(query=Q.transpose(1, 2)), "query must be"), (dict(out=Q.float()), "out must"), (dict(out=Q[:2]), "out must"),
+])
+def test_attention_refuses_what_does_not_fit(change, what):
+    with pytest.raises(RuntimeError, match=what):
+        _attend(**change)
+
+
+def test_what_is_no_tensor_is_a_type_error():
+    with pytest.raises(TypeError, match="lengths"):
+        _attend(lengths=[1, 1, 1])
+    with pytest.raises(TypeError, match="key_exponents"):
+        _attend(key_exponents=3)
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(), "CUDA"), (dict(positions=torch.zeros(2, dtype=torch.int32)), "positions"), (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions"),
+    (dict(key=Q.view(3, 256)), "key"), (dict(key=Q.view(3, 256)[:2].bfloat16()), "key must have"), (dict(head_size=48), "query must be"),
+    (dict(head_size=0), "query must be"), (dict(query=Q[:2, :, ::2].flatten(1)[:, ::2]), "query must be"),
+    (dict(cos_sin_cache=torch.zeros(8, 64, dtype=torch.float64)), "cos_sin_cache"), (dict(cos_sin_cache=torch.zeros(8, 128)[:, ::2]), "cos_sin_cache"),
+    (dict(query_weight=torch.zeros(32, dtype=torch.float16)), "weight"), (dict(key_weight=torch.zeros(64)), "weight"),
+    (dict(query_out=Q.view(3, 256)), "query_out"), (dict(key_out=Q.view(3, 256)), "key_out"),
+])
+def test_norm_and_rotation_refuse_what_does_not_fit(change, what):
+    a = dict(positions=torch.zeros(2, dtype=torch.int64), query=Q[:2].flatten(1).clone(), key=Q[:2].flatten(1).clone(), head_size=64,
+             cos_sin_cache=torch.zeros(8, 64), is_neox=True) | change
+    with pytest.raises(RuntimeError, match=what):
+        capi.qk_norm_rotary_embedding(**a)
+
+
+def test_a_missing_binding_fails_loudly(monkeypatch):
+    import sys
+
+    import triteia_b200
+
+    monkeypatch.setitem(sys.modules, "triteia_b200._binding", None)      # what an import that finds nothing leaves
+    monkeypatch.delattr(triteia_b200, "_binding", raising=False)
+    with pytest.raises(ImportError, match="no CPU"):
+        _lib.load_binding()

@@ -507,7 +507,7 @@ def test_refusals_on_the_device(cuda):
             ops.paged_attention(**a)
     with pytest.raises(RuntimeError, match="slots"):
         ops.cache_write(b.kc[0], b.vc[0], b.kc, b.vc, torch.zeros(16, dtype=torch.int32, device="cuda"))
-    with pytest.raises(RuntimeError, match="slots for"):
+    with pytest.raises(RuntimeError, match="slots"):
         ops.cache_write(b.kc[0], b.vc[0], b.kc, b.vc, torch.zeros(15, dtype=torch.int64, device="cuda"))
     with pytest.raises(RuntimeError, match="No suitable kernel"):
         ops.cache_read(b.kc, b.vc, torch.zeros(1, dtype=torch.int64, device="cuda"), dtype=torch.float32)

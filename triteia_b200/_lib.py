@@ -120,3 +120,13 @@ def dtype_tag(dtype):
     if dtype == torch.bfloat16:
         return TRB_BF16
     raise RuntimeError(f"No suitable kernel. dtype={dtype}")
+
+
+def load_binding():
+    """The extension module with the operators whose calls are short (csrc/binding.cpp); no fallback either."""
+    try:
+        from . import _binding
+    except ImportError as e:
+        raise ImportError("triteia_b200/_binding.so is missing or does not load: run `python -m triteia_b200.build` "
+                          "(there is no CPU or PyTorch fallback)") from e
+    return _binding

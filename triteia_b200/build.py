@@ -3,16 +3,20 @@
     python -m triteia_b200.build
 
 produces triteia_b200/libtriteia_b200.so from triteia_b200/csrc/triteia_b200.cu (a single
-translation unit).  nvcc cross-compiles without a GPU.
+translation unit; nvcc cross-compiles without a GPU) and triteia_b200/_binding.so, the Python binding
+of the latency-critical operators, from triteia_b200/csrc/binding.cpp (g++ with torch's headers).
 """
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG, "csrc", "triteia_b200.cu")
 LIB = os.path.join(PKG, "libtriteia_b200.so")
+BINDING_SRC = os.path.join(PKG, "csrc", "binding.cpp")
+BINDING = os.path.join(PKG, "_binding.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -34,8 +38,30 @@ def needs_build():
     return any(os.path.getmtime(p) > t for p in sources() + [hdr])
 
 
+def build_binding(force=False):
+    """The extension module triteia_b200._binding; it finds libtriteia_b200.so next to itself."""
+    hdr = os.path.join(PKG, "..", "include", "triteia_b200.h")
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(BINDING) >= os.path.getmtime(p) for p in (BINDING_SRC, hdr)):
+        return BINDING
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           + [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
+           + [BINDING_SRC, "-o", BINDING, f"-L{PKG}", "-ltriteia_b200", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",
+              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed building _binding.so")
+    return BINDING
+
+
 def build(force=False, verbose=False):
     if not force and not needs_build():
+        build_binding()
         return LIB
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + [SRC, "-o", LIB]
@@ -45,6 +71,7 @@ def build(force=False, verbose=False):
         raise RuntimeError("nvcc failed building libtriteia_b200.so")
     if verbose:
         sys.stderr.write(res.stderr)
+    build_binding(force)
     return LIB
 
 

@@ -11,6 +11,8 @@ import torch
 from . import _lib
 from ._lib import lib, ptr, stream_of, dev_of
 
+_binding = _lib.load_binding()
+
 
 def _check_input(t, name):
     if not t.is_cuda:
@@ -181,50 +183,10 @@ def batched_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is
     _rotary(positions, query, key, head_size, cos_sin_cache, is_neox, rot_dim, cos_sin_cache_offsets)
 
 
-def _head_rows(t, name, head_size, like):
-    """(rows as a 2-D view, number of heads) of a [..., heads * head_size] tensor whose rows may be strided."""
-    if t.device != like.device or t.dtype != like.dtype:
-        raise RuntimeError(f"{name} must have the device and dtype of query ({like.device}, {like.dtype})")
-    if t.dim() != 2:
-        t = t.view(-1, t.size(-1))
-    if t.stride(1) != 1 or t.size(1) % head_size != 0:
-        raise RuntimeError(f"{name} must be [tokens, heads * {head_size}] with contiguous rows")
-    return t, t.size(1) // head_size
-
-
 def qk_norm_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight=None, key_weight=None,
                              eps=1e-6, query_out=None, key_out=None):
     """Root-mean-square norm of every head of query and key (weights [head_size] or None), then rotary_embedding, one pass.
     In place, or into query_out / key_out.  query [..., num_heads * head_size] and key [..., num_kv_heads * head_size] may be
     column ranges of a fused projection; cos_sin_cache [max_position, rot_dim] has query's dtype or float32.  A token whose
     position lies outside the cache is left alone."""
-    dev = dev_of(query)
-    query, num_heads = _head_rows(query, "query", head_size, query)
-    T = query.size(0)
-    q_out = query if query_out is None else _head_rows(query_out, "query_out", head_size, query)[0]
-    num_kv_heads, k_out = 0, None
-    if key is not None:
-        key, num_kv_heads = _head_rows(key, "key", head_size, query)
-        k_out = key if key_out is None else _head_rows(key_out, "key_out", head_size, query)[0]
-        if key.size(0) != T or k_out.shape != key.shape:
-            raise RuntimeError("key and key_out must have one row per row of query and the same heads")
-    if q_out.shape != query.shape or positions.numel() != T:
-        raise RuntimeError("positions and query_out must have one entry and one row per row of query")
-    if positions.dtype != torch.int64 or not positions.is_contiguous():
-        raise RuntimeError("positions must be a contiguous int64 tensor")
-    if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous() or cos_sin_cache.dtype not in (query.dtype, torch.float32):
-        raise RuntimeError("cos_sin_cache must be a contiguous [max_position, rot_dim] tensor of query's dtype or float32")
-    for w, n in ((query_weight, "query_weight"), (key_weight, "key_weight")):
-        if w is not None and (w.dtype != query.dtype or w.numel() != head_size or not w.is_contiguous() or w.device != query.device):
-            raise RuntimeError(f"{n} must be a contiguous [{head_size}] tensor of query's dtype and device")
-    if positions.device != query.device or cos_sin_cache.device != query.device:
-        raise RuntimeError("positions and cos_sin_cache must be on the device of query")
-    err = lib.trb_qk_norm_rotary(ptr(positions), ptr(query), ptr(q_out), ptr(key), ptr(k_out), ptr(query_weight), ptr(key_weight),
-                                 ptr(cos_sin_cache), int(cos_sin_cache.dtype == torch.float32), cos_sin_cache.size(0), T,
-                                 cos_sin_cache.size(1), query.stride(0), q_out.stride(0), 0 if key is None else key.stride(0),
-                                 0 if key is None else k_out.stride(0), num_heads, num_kv_heads, head_size, float(eps),
-                                 int(bool(is_neox)), _lib.dtype_tag(query.dtype), dev, stream_of(query))
-    if err == _lib.ERR_PROB_SHAPE:
-        raise RuntimeError(f"No suitable kernel. head_size={head_size} rot_dim={cos_sin_cache.size(1)} (head_size: a multiple of 8 up "
-                           "to 256, rot_dim even and at most head_size, rows on 16-byte boundaries)")
-    _lib.check(err, "qk_norm_rotary_embedding")
+    _binding.qk_norm_rotary(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight, key_weight, eps, query_out, key_out)
