@@ -36,6 +36,7 @@ struct AttnArgs {
   long long table_stride, num_pages;
   float scale_log2;                   // scale * log2(e)
   int tokens, seqs, kv_heads, group, page_size, table_width;
+  int page_shift;                     // log2(page_size), -1 where that is no integer
   int causal, window;
 };
 
@@ -119,14 +120,16 @@ struct AttnCfg {
   static constexpr int M = ROWS ? 64 : 16;
   static constexpr int ROWB = FP8 ? D : 2 * D;                  // bytes of a token's key or value
   static constexpr int CHUNKS = ROWB / 16;
-  static constexpr int UNIT = 64;                               // tokens of a stage, 16 loaded by each warp
+  static constexpr int NT = ROWS ? 4 : FP8 ? 2 : 1;             // a warp takes 16 * NT tokens at a time
+  static constexpr int UNIT = ROWS ? 64 : 64 * NT;              // tokens of a stage, a quarter loaded by each warp
+  static constexpr int WTOK = UNIT / 4;
   static constexpr int HALF_BYTES = UNIT * ROWB;                // keys; the values follow
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
   // About 96 KB of loads in flight per CTA and two CTAs per SM: 6.5 TB/s for about 1.5 us of latency is 66 KB per SM.
   static constexpr int STAGES = 98304 / STAGE_BYTES > 6 ? 6 : 98304 / STAGE_BYTES;
-  static constexpr int MASK_OFF = STAGES * STAGE_BYTES;         // uint16 [STAGES][4]: tokens that count
-  static constexpr int EXP_OFF = MASK_OFF + STAGES * 8;         // uint8 [STAGES][2][64]: exponents of keys and values
-  static constexpr int ML_OFF = EXP_OFF + (FP8 ? STAGES * 2 * UNIT : 0);   // float [M][2]: the CTA's maxima and sums
+  static constexpr int MASK_OFF = STAGES * STAGE_BYTES;         // uint32 [STAGES][4]: tokens that count, per loading warp
+  static constexpr int EXP_OFF = MASK_OFF + STAGES * 16;        // float [STAGES][3][UNIT]: 2^e of keys; e and 2^-e of values
+  static constexpr int ML_OFF = EXP_OFF + (FP8 ? STAGES * 3 * UNIT * 4 : 0);   // float [M][2]: the CTA's maxima and sums
   static constexpr int WML_OFF = ML_OFF + M * 8;                // float [4][16][2]: the warps' (M = 16)
   static constexpr int SMEM_BYTES = WML_OFF + 4 * 16 * 8;
   static constexpr int O_STRIDE = D + 4;                        // floats; rows of the joined states (in the idle ring)
@@ -221,7 +224,7 @@ struct AttnBias { static constexpr float value = std::is_same<TM, __half>::value
 // 16 rows x (16 * NT) tokens: scores, masks, running maxima, weights, product with the values.
 template <class T, class Cfg, int NT>
 __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t (&q)[Cfg::D / 16][4], const float (&c_row)[2],
-                                           uint32_t kbase, uint32_t vbase, const uint8_t* exps, unsigned long long valid, int j0,
+                                           uint32_t kbase, uint32_t vbase, const float* exps, unsigned long long valid, int j0,
                                            const int (&row_hi)[2], const int (&row_lo)[2], bool need_mask, int lane) {
   using TM = typename AttnMma<T, Cfg::FP8>::type;
   constexpr int D = Cfg::D, ROWB = Cfg::ROWB;
@@ -261,21 +264,17 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
   }
   // ---- scale.  With exponents the weight that meets the code of v_j is 2^(t_j - m), t_j = log2 weight + e_j, and m
   // runs over the t_j: the weights fit the MMA type whatever the values' magnitudes; the sum takes the 2^-e_j back out.
-  float ev[2 * NT][2], iv[2 * NT][2];
+  float2 iv[2 * NT];
   if constexpr (Cfg::FP8) {
 #pragma unroll
     for (int n = 0; n < 2 * NT; ++n) {
-      const uint32_t kb = *reinterpret_cast<const uint16_t*>(exps + n * 8 + 2 * quad);
-      const uint32_t vb = *reinterpret_cast<const uint16_t*>(exps + Cfg::UNIT + n * 8 + 2 * quad);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float kf = pow2_of_byte((kb >> (8 * e)) & 255);
-        const int vbyte = (vb >> (8 * e)) & 255;
-        ev[n][e] = (float)(vbyte - 127);
-        iv[n][e] = pow2_of_byte(254 - vbyte);
-        s[n][e] = fmaf(s[n][e] * kf, c_row[0], ev[n][e]);
-        s[n][2 + e] = fmaf(s[n][2 + e] * kf, c_row[1], ev[n][e]);
-      }
+      const float2 kf = *reinterpret_cast<const float2*>(exps + n * 8 + 2 * quad);
+      const float2 ev = *reinterpret_cast<const float2*>(exps + Cfg::UNIT + n * 8 + 2 * quad);
+      iv[n] = *reinterpret_cast<const float2*>(exps + 2 * Cfg::UNIT + n * 8 + 2 * quad);
+      s[n][0] = fmaf(s[n][0] * kf.x, c_row[0], ev.x);
+      s[n][1] = fmaf(s[n][1] * kf.y, c_row[0], ev.y);
+      s[n][2] = fmaf(s[n][2] * kf.x, c_row[1], ev.x);
+      s[n][3] = fmaf(s[n][3] * kf.y, c_row[1], ev.y);
     }
   } else {
 #pragma unroll
@@ -328,7 +327,7 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
     for (int e = 0; e < 4; ++e) {
       const float p = exp2_fast(s[n][e] - base[e >> 1]);
       s[n][e] = p;
-      if constexpr (Cfg::FP8) st.l[e >> 1] = fmaf(p, iv[n][e & 1], st.l[e >> 1]);
+      if constexpr (Cfg::FP8) st.l[e >> 1] = fmaf(p, e & 1 ? iv[n].y : iv[n].x, st.l[e >> 1]);
       else st.l[e >> 1] += p;
     }
   // ---- values: the weights are rounded to the MMA type (half a step, of random sign), the sum above is not.
@@ -387,52 +386,80 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
   const uint8_t* kc = static_cast<const uint8_t*>(a.key_cache);
   const uint8_t* vc = static_cast<const uint8_t*>(a.value_cache);
   constexpr int ESZ = Cfg::FP8 ? 1 : 2;
-  uint16_t* masks = reinterpret_cast<uint16_t*>(smem + Cfg::MASK_OFF);
-  uint8_t* exps = smem + Cfg::EXP_OFF;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Cfg::MASK_OFF);
+  float* exps = reinterpret_cast<float*>(smem + Cfg::EXP_OFF);
+  constexpr int WTOK = Cfg::WTOK;                     // 16 or 32 tokens of a stage are this warp's to load
+  const int tok = warp * WTOK + (lane & (WTOK - 1));  // this lane's among the unit's
 
-  // Page of this lane's token of unit u (0 <= the result < num_pages, or -1), asked for one unit ahead of the loads.
-  auto page_of = [&](int u) -> int {
-    const int j = u * Cfg::UNIT + warp * 16 + (lane & 15);
-    if (u >= u1 || j < lo || j >= hi) return -1;
-    const int pg = table[j / a.page_size];
-    return pg >= 0 && pg < a.num_pages ? pg : -1;
+  // Page and place of this lane's token of unit u (page -1: not visible, or not in the cache), found one unit ahead.
+  struct Where { int page, place; };
+  auto where = [&](int u) -> Where {
+    const int j = u * Cfg::UNIT + tok;
+    if (u >= u1 || j < lo || j >= hi) return {-1, 0};
+    const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+    const int pg = table[p];
+    return {pg >= 0 && pg < a.num_pages ? pg : -1, j - p * a.page_size};
   };
-  int ahead = page_of(u0);
-  int exp_reg = 127, exp_slot = -1;     // e4m3: the byte that the last issue() asked for, and where it belongs
+  Where ahead = where(u0);
+  int exp_slot = -1, kb = 127, vb = 127;              // e4m3: the bytes that the last issue() asked for, and their stage
   auto settle_exps = [&]() {
-    if (Cfg::FP8 && exp_slot >= 0) exps[(exp_slot * 2 + (lane >> 4)) * Cfg::UNIT + warp * 16 + (lane & 15)] = (uint8_t)exp_reg;
+    if (exp_slot >= 0 && lane < WTOK) {
+      float* e = exps + exp_slot * 3 * Cfg::UNIT + tok;
+      e[0] = pow2_of_byte(kb);
+      e[Cfg::UNIT] = (float)(vb - 127);
+      e[2 * Cfg::UNIT] = pow2_of_byte(254 - vb);
+    }
   };
-  // Loads this warp's 16 tokens of unit u into `slot`.
+  constexpr int PER = 32 / Cfg::CHUNKS;               // rows per instruction
+  const int c = lane % Cfg::CHUNKS, r0 = lane / Cfg::CHUNKS;
+  const long long row_bytes = a.c_tok * ESZ;
+  const bool paged16 = (a.page_size & 15) == 0;       // 16 tokens of a unit lie on one page
+  // Loads this warp's tokens of unit u into `slot`.
   auto issue = [&](int u, int slot) {
     if constexpr (Cfg::FP8) settle_exps();
-    const int pg = ahead;
-    ahead = page_of(u + 1);
+    const Where w = ahead;
+    ahead = where(u + 1);
     if (u < u1) {
-      const int j = u * Cfg::UNIT + warp * 16 + (lane & 15);
-      const bool there = pg >= 0;
-      const int place = there ? j % a.page_size : 0;
-      const long long off = there ? ((long long)pg * a.c_page + place * a.c_tok + kvh * a.c_head) * ESZ : 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
-      if (lane == 0) masks[slot * 4 + warp] = (uint16_t)mask;
+      const bool there = w.page >= 0;
+      long long off = there ? (long long)w.page * a.c_page + (long long)w.place * a.c_tok + (long long)kvh * a.c_head : 0;
+      if constexpr (ESZ == 2) off *= 2;
+      unsigned mask = __ballot_sync(0xffffffffu, there);
+      if constexpr (WTOK == 16) mask &= 0xffffu;
+      if (lane == 0) masks[slot * 4 + warp] = mask;
       if constexpr (Cfg::FP8) {
         exp_slot = slot;
-        exp_reg = 127;
+        kb = vb = 127;
         if (there) {
-          const long long eo = (long long)pg * a.e_page + place * a.e_tok + kvh * a.e_head;
-          exp_reg = lane < 16 ? a.key_exp[eo] : a.value_exp[eo];
+          const long long eo = (long long)w.page * a.e_page + (long long)w.place * a.e_tok + (long long)kvh * a.e_head;
+          kb = a.key_exp[eo];
+          vb = a.value_exp[eo];
         }
       }
-      constexpr int PER = 32 / Cfg::CHUNKS;       // rows per instruction
       const uint32_t dst = smem_base + slot * Cfg::STAGE_BYTES;
-      const int c = lane % Cfg::CHUNKS;
+      if (paged16 && mask == (WTOK == 16 ? 0xffffu : 0xffffffffu)) {
 #pragma unroll
-      for (int i = 0; i < 16 / PER; ++i) {
-        const int r = i * PER + lane / Cfg::CHUNKS;
-        const long long ro = __shfl_sync(0xffffffffu, off, r) + c * 16;
-        const bool ok = (mask >> r) & 1;
-        const uint32_t at = dst + attn_swizzle<Cfg::ROWB>(warp * 16 + r, c);
-        cp_async16(at, kc + ro, ok);
-        cp_async16(at + Cfg::HALF_BYTES, vc + ro, ok);
+        for (int g = 0; g < WTOK / 16; ++g) {
+          const long long base = __shfl_sync(0xffffffffu, off, g * 16) + r0 * row_bytes + c * 16;
+          const uint8_t *kp = kc + base, *vp = vc + base;
+#pragma unroll
+          for (int i = 0; i < 16 / PER; ++i) {
+            const uint32_t at = dst + attn_swizzle<Cfg::ROWB>(warp * WTOK + g * 16 + i * PER + r0, c);
+            cp_async16(at, kp, true);
+            cp_async16(at + Cfg::HALF_BYTES, vp, true);
+            kp += PER * row_bytes;
+            vp += PER * row_bytes;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < WTOK / PER; ++i) {
+          const int r = i * PER + r0;
+          const long long ro = __shfl_sync(0xffffffffu, off, r) + c * 16;
+          const bool ok = (mask >> r) & 1;
+          const uint32_t at = dst + attn_swizzle<Cfg::ROWB>(warp * WTOK + r, c);
+          cp_async16(at, kc + ro, ok);
+          cp_async16(at + Cfg::HALF_BYTES, vc + ro, ok);
+        }
       }
     } else {
       exp_slot = -1;
@@ -514,18 +541,18 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
     else __syncwarp();
     issue(u + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
     if (!idle) {
-      constexpr int NT = Cfg::ROWS ? 4 : 1;
-      constexpr int TOK = NT * 16;
-      const int own = Cfg::ROWS ? 0 : warp * 16;
+      constexpr int TOK = Cfg::NT * 16;
+      const int own = Cfg::ROWS ? 0 : warp * WTOK;
       const int j0 = u * Cfg::UNIT + own;
-      const unsigned long long valid = Cfg::ROWS ? *reinterpret_cast<const unsigned long long*>(masks + slot * 4)
-                                                 : (unsigned long long)masks[slot * 4 + warp];
-      constexpr unsigned long long kAll = Cfg::ROWS ? ~0ull : 0xffffull;
+      const uint32_t* mk = masks + slot * 4;
+      const unsigned long long valid =
+          Cfg::ROWS ? (unsigned long long)(mk[0] | mk[1] << 16) | (unsigned long long)(mk[2] | mk[3] << 16) << 32 : mk[warp];
+      constexpr unsigned long long kAll = ~0ull >> (64 - TOK);
       if (valid != 0) {
         const bool need_mask = valid != kAll || j0 + TOK > all_hi || j0 < all_lo;
-        const uint32_t kb = smem_base + slot * Cfg::STAGE_BYTES + own * Cfg::ROWB;
-        attn_block<T, Cfg, NT>(st, q, c_row, kb, kb + Cfg::HALF_BYTES, exps + slot * 2 * Cfg::UNIT + own, valid, j0, row_hi, row_lo,
-                               need_mask, lane);
+        const uint32_t kbase = smem_base + slot * Cfg::STAGE_BYTES + own * Cfg::ROWB;
+        attn_block<T, Cfg, Cfg::NT>(st, q, c_row, kbase, kbase + Cfg::HALF_BYTES, exps + slot * 3 * Cfg::UNIT + own, valid, j0, row_hi,
+                                    row_lo, need_mask, lane);
       }
     }
     if constexpr (!Cfg::ROWS) __syncwarp();
@@ -617,16 +644,24 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
   if (parts > 1) cluster_sync_all();    // nobody's shared memory goes before its neighbours have read it
 }
 
-// CTAs of a cluster that share a tile.
-static int attn_parts(long long tiles, long long most_tokens, int sms) {
-  int parts = 1;
-  while (parts < 8 && tiles * parts < 4LL * sms && 2LL * parts * 128 <= most_tokens) parts *= 2;
-  return parts;
+// CTAs of a cluster that share a tile: where the tiles alone would leave SMs idle (two CTAs fit an SM), as many as fill
+// one wave, at most 16; several waves of tiles are cut into eight or so, so that sequences of different lengths even out.
+static int attn_parts(long long tiles, long long most_tokens, int unit, int sms) {
+  const long long slots = 2LL * sms, units = (most_tokens + unit - 1) / unit;
+  long long parts = 2 * tiles <= slots ? slots / tiles : (8 * slots + tiles - 1) / tiles;
+  parts = parts > 16 ? 16 : parts;
+  if (2 * tiles > slots && parts > 8) parts = 8;
+  if (parts > (units + 1) / 2) parts = (units + 1) / 2;      // two units each at least
+  return parts < 1 ? 1 : (int)parts;
 }
 
 template <class T, class Cfg>
 static int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
-  static std::atomic<bool> done[64];
+  static std::atomic<bool> wide[64], done[64];
+  if (dev < 0 || dev >= 64 || !wide[dev].load(std::memory_order_acquire)) {      // clusters of more than eight CTAs
+    if (cudaFuncSetAttribute(attn_kernel<T, Cfg>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return TRB_ERR_CUDA;
+    if (dev >= 0 && dev < 64) wide[dev].store(true, std::memory_order_release);
+  }
   if (!ensure_smem_attr(attn_kernel<T, Cfg>, dev, Cfg::SMEM_BYTES, done)) return TRB_ERR_CUDA;
   const long long rows = (long long)a.tokens * a.group;
   const long long per_token = (a.group + Cfg::M - 1) / Cfg::M;
@@ -635,7 +670,7 @@ static int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
   long long tiles = a.query_starts ? rows / Cfg::M + a.seqs : a.seqs * per_token;
   if (a.query_starts && tiles > a.tokens * per_token) tiles = a.tokens * per_token;
   if (tiles == 0) return TRB_OK;
-  const int parts = attn_parts(tiles * a.kv_heads, (long long)a.table_width * a.page_size, sm_count(dev));
+  const int parts = attn_parts(tiles * a.kv_heads, (long long)a.table_width * a.page_size, Cfg::UNIT, sm_count(dev));
   const long long grid = tiles * a.kv_heads * parts;
   if (grid > 0x7fffffffLL) return TRB_ERR_PROB_SHAPE;
   cudaLaunchConfig_t cfg = {};
@@ -656,57 +691,4 @@ static int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
   return TRB_OK;
 }
 
-template <class T>
-static int launch_attn(const AttnArgs& a, int head_size, int dev, cudaStream_t st) {
-  // Rows of an average sequence: up to 16 the warps of a CTA split the tokens, beyond that the rows.
-  const bool rows = a.query_starts ? (long long)a.tokens * a.group > 16LL * a.seqs : a.group > 16;
-  const bool fp8 = a.key_exp != nullptr;
-#define TRB_ATTN(F, DD, R) return launch_attn<T, AttnCfg<T, F, DD, R>>(a, dev, st)
-  if (head_size == 128) {
-    if (fp8) { if (rows) TRB_ATTN(true, 128, true); else TRB_ATTN(true, 128, false); }
-    if (rows) TRB_ATTN(false, 128, true);
-    TRB_ATTN(false, 128, false);
-  }
-  if (fp8) { if (rows) TRB_ATTN(true, 64, true); else TRB_ATTN(true, 64, false); }
-  if (rows) TRB_ATTN(false, 64, true);
-  TRB_ATTN(false, 64, false);
-#undef TRB_ATTN
-}
-
 }  // namespace trb
-
-extern "C" int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
-                                   const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,
-                                   void* out, int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size, int page_size,
-                                   long long num_pages, long long table_stride, int table_width, long long query_token_stride,
-                                   long long query_head_stride, long long out_token_stride, long long out_head_stride,
-                                   long long page_stride, long long token_stride, long long head_stride, long long exp_page_stride,
-                                   long long exp_token_stride, long long exp_head_stride, float scale, int causal, int window, int dtype,
-                                   int dev, void* stream) {
-  using namespace trb;
-  if (num_tokens == 0 || num_seqs == 0) return TRB_OK;
-  const bool fp8 = key_exponents != nullptr;
-  if (num_tokens < 0 || num_seqs < 0 || !query || !key_cache || !value_cache || !lengths || !out || fp8 != (value_exponents != nullptr) ||
-      num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0) || window < 0)
-    return TRB_ERR_BAD_ARG;
-  if (!query_starts && num_tokens != num_seqs) return TRB_ERR_BAD_ARG;
-  if (num_heads % num_kv_heads != 0 || (window > 0 && !causal)) return TRB_ERR_PROB_SHAPE;
-  const int esz = fp8 ? 1 : 2;
-  if (((uintptr_t)query | (uintptr_t)out | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15) return TRB_ERR_PROB_SHAPE;
-  if ((query_token_stride | query_head_stride | out_token_stride | out_head_stride) & 7) return TRB_ERR_PROB_SHAPE;
-  if (((page_stride | token_stride | head_stride) * esz) & 15) return TRB_ERR_PROB_SHAPE;
-  // Positions are 32-bit numbers; the largest unit starts below length + 64.
-  if ((long long)table_width * page_size > 0x7fff0000LL || (long long)num_tokens * (num_heads / num_kv_heads) > 0x7fff0000LL)
-    return TRB_ERR_PROB_SHAPE;
-  if (dtype != TRB_F16 && dtype != TRB_BF16) return TRB_ERR_KERN_SHAPE;
-  if (head_size != 64 && head_size != 128) return TRB_ERR_KERN_SHAPE;
-  DeviceGuard guard(dev);
-  if (!guard.ok) return TRB_ERR_CUDA;
-  const AttnArgs a{query, key_cache, value_cache, (const uint8_t*)key_exponents, (const uint8_t*)value_exponents,
-                   (const int*)page_table, (const int*)lengths, (const int*)query_starts, out, query_token_stride, query_head_stride,
-                   out_token_stride, out_head_stride, page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride,
-                   exp_head_stride, table_stride, num_pages, scale * 1.4426950408889634f, num_tokens, num_seqs, num_kv_heads,
-                   num_heads / num_kv_heads, page_size, table_width, causal, window};
-  if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, dev, (cudaStream_t)stream);
-  return launch_attn<__nv_bfloat16>(a, head_size, dev, (cudaStream_t)stream);
-}

@@ -1,0 +1,67 @@
+// Host side of paged attention: the choice of the kernel and the C entry point.
+#pragma once
+
+#include "attention_tc.cuh"
+
+namespace trb {
+
+template <class T>
+static int launch_attn(const AttnArgs& a, int head_size, int dev, cudaStream_t st) {
+  // Rows of an average sequence: up to 16 the warps of a CTA split the tokens, beyond that the rows.
+  const bool rows = a.query_starts ? (long long)a.tokens * a.group > 16LL * a.seqs : a.group > 16;
+  const bool fp8 = a.key_exp != nullptr;
+  // From 128 rows of an average sequence on the matrix products bound the call.
+  if ((long long)a.tokens * a.group >= 128LL * a.seqs && attn_tc_fits(a)) {
+    if (head_size == 128) return launch_attn_tc<T, 128>(a, dev, st);
+    return launch_attn_tc<T, 64>(a, dev, st);
+  }
+#define TRB_ATTN(F, DD, R) return launch_attn<T, AttnCfg<T, F, DD, R>>(a, dev, st)
+  if (head_size == 128) {
+    if (fp8) { if (rows) TRB_ATTN(true, 128, true); else TRB_ATTN(true, 128, false); }
+    if (rows) TRB_ATTN(false, 128, true);
+    TRB_ATTN(false, 128, false);
+  }
+  if (fp8) { if (rows) TRB_ATTN(true, 64, true); else TRB_ATTN(true, 64, false); }
+  if (rows) TRB_ATTN(false, 64, true);
+  TRB_ATTN(false, 64, false);
+#undef TRB_ATTN
+}
+
+}  // namespace trb
+
+extern "C" int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
+                                   const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,
+                                   void* out, int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size, int page_size,
+                                   long long num_pages, long long table_stride, int table_width, long long query_token_stride,
+                                   long long query_head_stride, long long out_token_stride, long long out_head_stride,
+                                   long long page_stride, long long token_stride, long long head_stride, long long exp_page_stride,
+                                   long long exp_token_stride, long long exp_head_stride, float scale, int causal, int window, int dtype,
+                                   int dev, void* stream) {
+  using namespace trb;
+  if (num_tokens == 0 || num_seqs == 0) return TRB_OK;
+  const bool fp8 = key_exponents != nullptr;
+  if (num_tokens < 0 || num_seqs < 0 || !query || !key_cache || !value_cache || !lengths || !out || fp8 != (value_exponents != nullptr) ||
+      num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0) || window < 0)
+    return TRB_ERR_BAD_ARG;
+  if (!query_starts && num_tokens != num_seqs) return TRB_ERR_BAD_ARG;
+  if (num_heads % num_kv_heads != 0 || (window > 0 && !causal)) return TRB_ERR_PROB_SHAPE;
+  const int esz = fp8 ? 1 : 2;
+  if (((uintptr_t)query | (uintptr_t)out | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15) return TRB_ERR_PROB_SHAPE;
+  if ((query_token_stride | query_head_stride | out_token_stride | out_head_stride) & 7) return TRB_ERR_PROB_SHAPE;
+  if (((page_stride | token_stride | head_stride) * esz) & 15) return TRB_ERR_PROB_SHAPE;
+  // Positions are 32-bit numbers; the largest unit starts below length + 64.
+  if ((long long)table_width * page_size > 0x7fff0000LL || (long long)num_tokens * (num_heads / num_kv_heads) > 0x7fff0000LL)
+    return TRB_ERR_PROB_SHAPE;
+  if (dtype != TRB_F16 && dtype != TRB_BF16) return TRB_ERR_KERN_SHAPE;
+  if (head_size != 64 && head_size != 128) return TRB_ERR_KERN_SHAPE;
+  DeviceGuard guard(dev);
+  if (!guard.ok) return TRB_ERR_CUDA;
+  const AttnArgs a{query, key_cache, value_cache, (const uint8_t*)key_exponents, (const uint8_t*)value_exponents,
+                   (const int*)page_table, (const int*)lengths, (const int*)query_starts, out, query_token_stride, query_head_stride,
+                   out_token_stride, out_head_stride, page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride,
+                   exp_head_stride, table_stride, num_pages, scale * 1.4426950408889634f, num_tokens, num_seqs, num_kv_heads,
+                   num_heads / num_kv_heads, page_size, table_width,
+                   (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1, causal, window};
+  if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, dev, (cudaStream_t)stream);
+  return launch_attn<__nv_bfloat16>(a, head_size, dev, (cudaStream_t)stream);
+}

@@ -1,0 +1,479 @@
+// Attention of new tokens over a paged cache on the fifth-generation tensor cores: the calls that the matrix products
+// bound (prompts, long chunks), with a cache of the inputs' type.  Definition and masks as in attention.cuh.
+//
+// A CTA owns 256 rows (token, query head of the group) of one sequence and key head, as two tiles of 128, and walks the
+// visible keys in tiles of 128.  While the tensor cores work on one tile, the other one's softmax runs:
+//   scores   S = Q K^T   tcgen05.mma, both operands K-major in shared memory, S fp32 in tensor memory (128 columns a tile)
+//   softmax  one thread per row: the row comes out of tensor memory into registers, no shuffle is needed; weights go back
+//            as 16-bit numbers into the same columns
+//   values   O += P V    A operand = the weights in tensor memory, B operand = V rows as they lie in memory (MN-major)
+// so scores and weights never touch shared memory.  O stays in tensor memory; it is rescaled only when a row's maximum
+// has grown by more than 2^8 since the last time (the weights are then at most 2^8 times what they would be, which fp32
+// sums and fp16 or bf16 weights hold), so almost never after the first tiles.
+//   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (TMEM lanes 32 * (warp % 4) ..)
+//   warp 8           issues the MMAs (an elected lane), owns the tensor memory
+//   warp 9           loads: one box per page and 64 sizes, a lane per page.  A page outside the cache, and boxes that no
+//                    row sees, become boxes past the end of the cache, which TMA fills with zeros.
+//   warps 10, 11     complete the third warpgroup, which hands registers to the other two
+// Order of the MMAs: S0(0) S1(0), then for every key tile O0 += P0 V, S0(next), O1 += P1 V, S1(next): S(next) of a tile may
+// overwrite its P because the pipe runs in order, and when S(next) is complete so is that tile's O.
+//
+// Shared memory: 64 KB of queries and a ring of five 32 KB tiles (K0, V0, K1, ..); 512 tensor memory columns: S, O of both.
+#pragma once
+
+#include "attention.cuh"
+
+namespace trb {
+
+template <int D_>
+struct AttnTcCfg {
+  static constexpr int D = D_;
+  static constexpr int HALVES = D / 64;                  // 128-byte swizzle atoms of a row
+  static constexpr int TILE_BYTES = 128 * D * 2;         // 128 rows of queries, keys or values
+  static constexpr int BUFS = 5;
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = 2 * TILE_BYTES;
+  static constexpr int BAR_OFF = KV_OFF + BUFS * TILE_BYTES;
+  static constexpr int NUM_BARS = 2 * BUFS + 1 + 3 * 2;
+  static constexpr int SMEM_BYTES = BAR_OFF + NUM_BARS * 8 + 16;
+  static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;
+  static constexpr int THREADS = 12 * 32;
+  // Registers a thread: the softmax warps hold a row of 128 scores, the third warpgroup needs few; together what the
+  // launch has, 3 x 168.
+  static constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 216, OTHER_REGS = 72;
+  static_assert(2 * SOFTMAX_REGS + OTHER_REGS <= 3 * LAUNCH_REGS, "the register split is covered by the launch");
+  static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr uint32_t S_COL = 0, O_COL = 256;      // tile t: S_COL + 128 t, O_COL + 128 t
+};
+static_assert(AttnTcCfg<128>::SMEM_ALLOC <= 232448, "shared memory of one CTA");
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_one(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D[128, N] (+)= A[128, 16] B[16, N]; A and B in shared memory.
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory: 8 columns of two 16-bit numbers per row.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+      "%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+// Two 32-bit multiply-adds in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+template <class T, class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a, int tiles_bound,
+               int box) {
+  constexpr int D = Cfg::D, BUFS = Cfg::BUFS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFF);   // a tile of keys or values has landed
+  uint64_t* empty_bar = full_bar + BUFS;                                   // its MMAs have retired
+  uint64_t* q_bar = empty_bar + BUFS;                                      // the queries are in shared memory
+  uint64_t* s_bar = q_bar + 1;                                             // [2] scores complete
+  uint64_t* p_bar = s_bar + 2;                                             // [2] weights stored
+  uint64_t* o_bar = p_bar + 2;                                             // [2] output complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_bar + 2);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // Late tiles of a causal prompt see the most keys: they go first.
+  const int kvh = blockIdx.x % a.kv_heads;
+  AttnTile t;
+  if (!attn_find_tile<256>(a, tiles_bound - 1 - (int)(blockIdx.x / a.kv_heads), t)) return;
+  int lo, hi;
+  attn_key_range(a, t, lo, hi);
+  // Key tiles [kt0, kt0 + n[i]) concern the rows of tile i.
+  const int kt0 = lo / 128;
+  const int base_pos = t.length - t.new_tokens;
+  int n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int rows = min(128, t.rows - 128 * i);
+    int h = hi;
+    if (a.causal && rows > 0) h = min(hi, base_pos + (t.row0 + 128 * i + rows - 1) / a.group + 1);
+    n[i] = rows > 0 && h > lo ? (h + 127) / 128 - kt0 : 0;
+  }
+  const int n_all = max(n[0], n[1]);
+
+  if (tid == 0) {
+    for (int i = 0; i < BUFS; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], 1);
+    }
+    mbar_init(q_bar, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_bar[i], 1);
+      mbar_init(&p_bar[i], 4);
+      mbar_init(&o_bar[i], 1);
+    }
+    *dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const uint32_t smem_base = smem_u32(smem);
+  const int* table = a.page_table + t.seq * a.table_stride;
+
+  if (warp >= 8) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::OTHER_REGS));
+   if (warp == 9) {
+    // ------------------------------ loads ------------------------------
+    const int boxes = 128 / box;                      // at most 8
+    const bool mine = lane < boxes;
+    if (lane == 0) {
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
+    int buf = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n_all; ++i) {
+      const int j = (kt0 + i) * 128 + lane * box;
+      int page = -1, place = 0;
+      if (mine && j < hi && j + box > lo) {
+        const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+        page = table[p];
+        place = j - p * a.page_size;
+      }
+      if (page < 0 || page >= a.num_pages) page = (int)a.num_pages;     // past the end: zeros
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        mbar_wait(&empty_bar[buf], phase ^ 1, dead);
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[buf], Cfg::TILE_BYTES);
+        __syncwarp();
+        if (mine) {
+          const uint32_t dst = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES + lane * box * 128;
+#pragma unroll
+          for (int h = 0; h < Cfg::HALVES; ++h) tma_load_4d(dst + h * 16384, kv ? &tm_v : &tm_k, h * 64, kvh, place, page, &full_bar[buf]);
+        }
+        if (++buf == BUFS) { buf = 0; phase ^= 1; }
+      }
+    }
+   } else if (warp == 8) {
+    // ------------------------------ MMAs ------------------------------
+    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+    auto scores = [&](int tile, int buf) {            // S[tile] = Q[tile] K^T
+      const uint64_t qd = tc_smem_desc(smem_base + Cfg::Q_OFF + tile * Cfg::TILE_BYTES);
+      const uint64_t kd = tc_smem_desc(smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {            // 32 bytes along a row; the next 64 sizes are 16 KB further
+          const uint64_t step = (uint64_t)((k >> 2) * (16384 >> 4) + (k & 3) * 2);
+          tc_mma_f16_ss(tmem + Cfg::S_COL + tile * 128, qd + step, kd + step, idesc_s, k > 0);
+        }
+        tc_commit_one(&s_bar[tile]);
+      }
+      __syncwarp();
+    };
+    auto outputs = [&](int tile, int buf, bool first, bool last) {      // O[tile] += P[tile] V
+      const uint32_t v = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES;
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)                   // 16 tokens = 16 rows of 128 bytes
+          tc_mma_f16_ts(tmem + Cfg::O_COL + tile * 128, tmem + Cfg::S_COL + tile * 128 + k * 8,
+                        tc_smem_desc_mn(v + k * 2048, 16384, 1024), idesc_o, !first || k > 0);
+        if (last) tc_commit_one(&o_bar[tile]);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int buf) {
+      if (elect_one()) tc_commit_one(&empty_bar[buf]);
+      __syncwarp();
+    };
+    // Items of the ring: K of key tile i is number 2i, V number 2i + 1.
+    auto landed = [&](int x) { mbar_wait(&full_bar[x % BUFS], (x / BUFS) & 1, dead); };
+    if (n_all > 0) {
+      mbar_wait(q_bar, 0, dead);
+      landed(0);
+      tc_fence_after();
+      for (int i = 0; i < 2; ++i)
+        if (n[i] > 0) scores(i, 0);
+      release(0);
+    }
+    for (int i = 0; i < n_all; ++i) {
+      const int vbuf = (2 * i + 1) % BUFS, kbuf = (2 * i + 2) % BUFS;
+      landed(2 * i + 1);
+      // Values of tokens that no row sees may be anything, and 0 * NaN is NaN: they become zeros.
+      const int j0 = (kt0 + i) * 128, from = max(0, lo - j0), to = min(128, hi - j0);
+      if (from > 0 || to < 128) {
+        const uint32_t v = smem_base + Cfg::KV_OFF + vbuf * Cfg::TILE_BYTES;
+        for (int x = lane; x < 128 * 8 * Cfg::HALVES; x += 32) {      // 16 bytes each
+          const int r = (x >> 3) & 127;
+          if (r < from || r >= to) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v + x * 16), "r"(0) : "memory");
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
+      const bool more = i + 1 < n_all;
+      for (int tile = 0; tile < 2; ++tile) {
+        if (i < n[tile]) {
+          mbar_wait(&p_bar[tile], i & 1, dead);
+          tc_fence_after();
+          outputs(tile, vbuf, i == 0, i + 1 == n[tile]);
+        }
+        if (more && tile == 0) landed(2 * i + 2);
+        if (i + 1 < n[tile]) scores(tile, kbuf);
+      }
+      release(vbuf);
+      if (more) release(kbuf);
+    }
+   }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::SOFTMAX_REGS));
+    // ------------------------------ softmax: a thread per row ------------------------------
+    const int tile = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;              // of the tile
+    const int trow = tile * 128 + row;                // of the work item
+    const bool on = trow < t.rows;
+    const int rq = t.row0 + (on ? trow : 0);
+    const int qi = rq / a.group, head = kvh * a.group + (rq - qi * a.group);
+    const uint32_t qtile = smem_base + Cfg::Q_OFF + tile * Cfg::TILE_BYTES;
+    // A negative scale turns the sign of the queries, so that the largest score is the largest product.
+    const float c = fmaxf(fabsf(a.scale_log2), 1e-35f);      // a scale of zero: masked scores stay -inf
+    {
+      const T* qp = static_cast<const T*>(a.query) + (t.q0 + qi) * a.q_tok + head * a.q_head;
+      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x) {
+        uint4 w = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t at = qtile + (x >> 3) * 16384 + row * 128 + (((x & 7) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x ^ flip), "r"(w.y ^ flip), "r"(w.z ^ flip), "r"(w.w ^ flip)
+                     : "memory");
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_bar);
+    }
+    const int pos = base_pos + qi;
+    const int row_hi = a.causal ? min(hi, pos + 1) : hi;
+    const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    // Tokens [all_lo, all_hi) are seen by every row of the warp.
+    const int first_row = t.row0 + tile * 128 + quarter * 32, last_row = t.row0 + min(tile * 128 + quarter * 32 + 31, t.rows - 1);
+    const int all_hi = a.causal ? min(hi, base_pos + first_row / a.group + 1) : hi;
+    const int all_lo = a.window > 0 ? base_pos + last_row / a.group - a.window + 1 : 0;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + Cfg::S_COL + tile * 128, o_addr = tmem + lanes + Cfg::O_COL + tile * 128;
+    constexpr float kBias = AttnBias<T>::value / 2;   // weights: at most 2^(8 + 4) in fp16
+    float m = -INFINITY, l = 0.f;
+
+    // Which of the 16-token groups of a key tile are in the cache (bit g); tokens that no row sees count as there.
+    auto groups_there = [&](int i) -> uint32_t {
+      bool there = true;
+      if (lane < 8) {
+        const int j = (kt0 + i) * 128 + lane * 16;
+        if (j < hi && j + 16 > lo) {
+          const int pg = table[a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size];
+          there = pg >= 0 && pg < a.num_pages;
+        }
+      }
+      return __ballot_sync(0xffffffffu, there);
+    };
+    uint32_t there_next = n[tile] > 0 ? groups_there(0) : 0u;
+    for (int i = 0; i < n[tile]; ++i) {
+      const uint32_t there = there_next;
+      if (i + 1 < n[tile]) there_next = groups_there(i + 1);
+      const int j0 = (kt0 + i) * 128;
+      mbar_wait(&s_bar[tile], i & 1, dead);
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) tc_ld32(s_addr + b * 32, v[b]);
+      tc_wait_ld();
+      if (there != 0xffffffffu || j0 + 128 > all_hi || j0 < all_lo) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const int j = j0 + b * 32 + x;
+            if (j >= row_hi || j < row_lo || !((there >> (b * 2 + (x >> 4))) & 1)) v[b][x] = 0xff800000u;   // -inf
+          }
+      }
+      float mx[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        mx[b] = __uint_as_float(v[b][0]);
+#pragma unroll
+        for (int x = 1; x < 32; ++x) mx[b] = fmaxf(mx[b], __uint_as_float(v[b][x]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;      // -inf * 0 is NaN, which fmaxf drops
+      const float m_new = fmaxf(m, top);
+      if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
+        if (i > 0) {
+          // This tile's S is complete, so its last O is too.
+          const float alpha = m == -INFINITY ? 1.f : exp2_fast(m - m_new);        // nothing in O yet: nothing to scale
+          l *= alpha;
+#pragma unroll
+          for (int b = 0; b < D / 32; ++b) {
+            uint32_t o[32];
+            tc_ld32(o_addr + b * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tc_st32(o_addr + b * 32, o);
+          }
+        }
+        m = m_new;
+      }
+      const float off = kBias - (m == -INFINITY ? 0.f : m);
+      const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const int b = h * 2 + (x >> 4), e = (x & 15) * 2;
+          float2 y = fma2(make_float2(__uint_as_float(v[b][e]), __uint_as_float(v[b][e + 1])), c2, off2);
+          y.x = exp2_fast(y.x);
+          y.y = exp2_fast(y.y);
+          sum.x += y.x;
+          sum.y += y.y;
+          p[x] = pack2(y.x, y.y, T());
+        }
+        tc_st32(s_addr + h * 32, p);
+      }
+      l += sum.x + sum.y;
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_bar[tile]);
+    }
+    // ------------------------------ epilogue ------------------------------
+    if (n[tile] > 0) {
+      mbar_wait(&o_bar[tile], 0, dead);
+      tc_fence_after();
+    } else {
+      mbar_wait(q_bar, 0, dead);                      // the staging rows below are the queries' rows
+    }
+    // Every MMA of this tile has retired: its queries' rows take the output on its way to whole rows in memory.
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t patch = qtile + quarter * (32 * D * 2);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) {
+      uint32_t o[32] = {};
+      if (n[tile] > 0) {
+        tc_ld32(o_addr + b * 32, o);
+        tc_wait_ld();
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = l == 0.f ? 0.f : __uint_as_float(o[x * 8 + e * 2]) * inv;
+          const float y1 = l == 0.f ? 0.f : __uint_as_float(o[x * 8 + e * 2 + 1]) * inv;
+          w[e] = pack2(y0, y1, T());
+        }
+        const uint32_t at = patch + attn_swizzle<D * 2>(lane, b * 4 + x);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      }
+    }
+    __syncwarp();
+    const long long out_at = on ? (long long)(t.q0 + qi) * a.o_tok + (long long)head * a.o_head : -1;
+    constexpr int CH = D / 8;                         // 16-byte pieces of a row
+#pragma unroll 4
+    for (int x = 0; x < CH; ++x) {
+      const int r = x * (32 / CH) + lane / CH, ch = lane % CH;
+      const long long at = __shfl_sync(0xffffffffu, out_at, r);
+      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + ch * 8) = lds128(patch + attn_swizzle<D * 2>(r, ch));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS) : "memory");
+  }
+}
+
+// The cache as (size, head, place, page), a box = 64 sizes of `box` tokens of one page and head, 128-byte swizzle.
+static bool make_map_cache(CUtensorMap* map, bool bf16, const void* base, const AttnArgs& a, int size, int box) {
+  auto fn = get_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.page_size, (cuuint64_t)a.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)a.c_head * 2, (cuuint64_t)a.c_tok * 2, (cuuint64_t)a.c_page * 2};
+  cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tokens of a TMA box: what divides both a page and a tile of 128 keys.
+static int attn_tc_box(int page_size) {
+  int box = page_size & -page_size;
+  return box > 128 ? 128 : box;
+}
+
+// Whether the tensor-memory kernel takes the call: a cache of the inputs' type on pages that hold whole groups of 16 tokens.
+static bool attn_tc_fits(const AttnArgs& a) {
+  if (a.key_exp != nullptr || a.query_starts == nullptr) return false;
+  if (attn_tc_box(a.page_size) < 16 || a.num_pages <= 0 || a.num_pages >= 0x7fffffffLL) return false;
+  if (a.c_head <= 0 || a.c_tok <= 0 || a.c_page <= 0) return false;
+  const long long most = 1LL << 38;                   // strides of a tensor map: below 2^40 bytes
+  return a.c_head < most && a.c_tok < most && a.c_page < most;
+}
+
+template <class T, int D>
+static int launch_attn_tc(const AttnArgs& a, int dev, cudaStream_t st) {
+  using Cfg = AttnTcCfg<D>;
+  static std::atomic<bool> done[64];
+  if (!ensure_smem_attr(attn_tc_kernel<T, Cfg>, dev, Cfg::SMEM_ALLOC, done)) return TRB_ERR_CUDA;
+  const int box = attn_tc_box(a.page_size);
+  CUtensorMap tk, tv;
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (!make_map_cache(&tk, bf16, a.key_cache, a, D, box) || !make_map_cache(&tv, bf16, a.value_cache, a, D, box)) return TRB_ERR_CUDA;
+  const long long per_token = (a.group + 255) / 256;
+  long long tiles = (long long)a.tokens * a.group / 256 + a.seqs;
+  if (tiles > a.tokens * per_token) tiles = a.tokens * per_token;
+  const long long grid = tiles * a.kv_heads;
+  if (grid > 0x7fffffffLL) return TRB_ERR_PROB_SHAPE;
+  attn_tc_kernel<T, Cfg><<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM_ALLOC, st>>>(tk, tv, a, (int)tiles, box);
+  return cudaGetLastError() == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
+}
+
+}  // namespace trb

@@ -19,4 +19,6 @@
 #include "qk_norm.cuh"
 #include "kv_cache.cuh"
 #include "attention.cuh"
+#include "attention_tc.cuh"
+#include "attention_host.cuh"
 #include "no_alloc.cuh"
