@@ -209,6 +209,12 @@ struct AttnMma { using type = T; };
 template <class T>
 struct AttnMma<T, true> { using type = __half; };
 
+// Exponent field of the power of two that brings a bf16 row with the largest magnitude `top` to 2^9 .. 2^10.
+__device__ __forceinline__ int attn_row_shift(float top) {
+  const int field = (int)(__float_as_uint(top) >> 23);                  // top in [2^(field - 127), twice that)
+  return top > 0.f ? min(max(127 + 127 + 9 - field, 1), 253) : 127;
+}
+
 // Softmax state of a warp's 16 rows; a lane has rows lane / 4 and lane / 4 + 8.
 template <int D>
 struct AttnState {
@@ -505,12 +511,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int field = (int)(__float_as_uint(top) >> 23);            // top in [2^(field - 127), twice that)
-        const int k = min(max(127 + 127 + 9 - field, 1), 253);          // exponent field of 2^(9 - exponent of top)
-        if (top > 0.f) {
-          up = __uint_as_float((uint32_t)k << 23);
-          c_row[rr] *= __uint_as_float((uint32_t)(254 - k) << 23);
-        }
+        const int k = attn_row_shift(top);
+        up = __uint_as_float((uint32_t)k << 23);
+        c_row[rr] *= __uint_as_float((uint32_t)(254 - k) << 23);
       }
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {

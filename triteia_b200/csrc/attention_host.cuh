@@ -12,8 +12,8 @@ static int launch_attn(const AttnArgs& a, int head_size, int dev, cudaStream_t s
   const bool fp8 = a.key_exp != nullptr;
   // From 128 rows of an average sequence on the matrix products bound the call.
   if ((long long)a.tokens * a.group >= 128LL * a.seqs && attn_tc_fits(a)) {
-    if (head_size == 128) return launch_attn_tc<T, 128>(a, dev, st);
-    return launch_attn_tc<T, 64>(a, dev, st);
+    if (head_size == 128) return fp8 ? launch_attn_tc<T, 128, true>(a, dev, st) : launch_attn_tc<T, 128, false>(a, dev, st);
+    return fp8 ? launch_attn_tc<T, 64, true>(a, dev, st) : launch_attn_tc<T, 64, false>(a, dev, st);
   }
 #define TRB_ATTN(F, DD, R) return launch_attn<T, AttnCfg<T, F, DD, R>>(a, dev, st)
   if (head_size == 128) {

@@ -18,34 +18,44 @@
 // Order of the MMAs: S0(0) S1(0), then for every key tile O0 += P0 V, S0(next), O1 += P1 V, S1(next): S(next) of a tile may
 // overwrite its P because the pipe runs in order, and when S(next) is complete so is that tile's O.
 //
-// Shared memory: 64 KB of queries and a ring of five 32 KB tiles (K0, V0, K1, ..); 512 tensor memory columns: S, O of both.
+// An e4m3 cache: the codes land in a ring of their own and four more warps (12-15) turn them into fp16 tiles, exactly; the
+// powers of two enter at the scores, as in attention.cuh: 2^(t_j - m) with t_j = log2 weight + e_j meets the code of v_j.
+// Queries and weights are fp16 there whatever T is (queries scaled by a power of two per row).
+//
+// Shared memory: 64 KB of queries and a ring of five 32 KB tiles (K0, V0, K1, ..) -- e4m3: three, and three of codes.
+// 512 tensor memory columns: S and O of both tiles.
 #pragma once
 
 #include "attention.cuh"
 
 namespace trb {
 
-template <int D_>
+template <int D_, bool FP8_>
 struct AttnTcCfg {
   static constexpr int D = D_;
+  static constexpr bool FP8 = FP8_;
   static constexpr int HALVES = D / 64;                  // 128-byte swizzle atoms of a row
   static constexpr int TILE_BYTES = 128 * D * 2;         // 128 rows of queries, keys or values
-  static constexpr int BUFS = 5;
+  static constexpr int BUFS = FP8 ? 3 : 5;
+  static constexpr int CODE_BYTES = 128 * D, CODE_BUFS = FP8 ? 3 : 0;
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
-  static constexpr int BAR_OFF = KV_OFF + BUFS * TILE_BYTES;
-  static constexpr int NUM_BARS = 2 * BUFS + 1 + 3 * 2;
+  static constexpr int CODE_OFF = KV_OFF + BUFS * TILE_BYTES;
+  static constexpr int EXP_OFF = CODE_OFF + CODE_BUFS * CODE_BYTES;      // float [2][3][128]: 2^e of keys; e and 2^-e of values
+  static constexpr int BAR_OFF = EXP_OFF + (FP8 ? 2 * 3 * 128 * 4 : 0);
+  static constexpr int NUM_BARS = 2 * BUFS + 1 + 3 * 2 + 2 * CODE_BUFS + 2;
   static constexpr int SMEM_BYTES = BAR_OFF + NUM_BARS * 8 + 16;
   static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;
-  static constexpr int THREADS = 12 * 32;
-  // Registers a thread: the softmax warps hold a row of 128 scores, the third warpgroup needs few; together what the
-  // launch has, 3 x 168.
-  static constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 216, OTHER_REGS = 72;
-  static_assert(2 * SOFTMAX_REGS + OTHER_REGS <= 3 * LAUNCH_REGS, "the register split is covered by the launch");
+  static constexpr int GROUPS = FP8 ? 4 : 3;             // warpgroups
+  static constexpr int THREADS = GROUPS * 128;
+  // Registers a thread: the softmax warps hold a row of 128 scores, the other warpgroups need few; together they stay
+  // within what the launch has.
+  static constexpr int LAUNCH_REGS = FP8 ? 128 : 168, SOFTMAX_REGS = FP8 ? 184 : 216, OTHER_REGS = 72;
+  static_assert(2 * SOFTMAX_REGS + (GROUPS - 2) * OTHER_REGS <= GROUPS * LAUNCH_REGS, "the register split is covered by the launch");
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t S_COL = 0, O_COL = 256;      // tile t: S_COL + 128 t, O_COL + 128 t
 };
-static_assert(AttnTcCfg<128>::SMEM_ALLOC <= 232448, "shared memory of one CTA");
+static_assert(AttnTcCfg<128, false>::SMEM_ALLOC <= 232448 && AttnTcCfg<128, true>::SMEM_ALLOC <= 232448, "shared memory of one CTA");
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
   asm volatile(
@@ -85,6 +95,20 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32])
       "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 // Two 32-bit multiply-adds in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -99,7 +123,8 @@ template <class T, class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a, int tiles_bound,
                int box) {
-  constexpr int D = Cfg::D, BUFS = Cfg::BUFS;
+  using TM = typename AttnMma<T, Cfg::FP8>::type;
+  constexpr int D = Cfg::D, BUFS = Cfg::BUFS, CODE_BUFS = Cfg::CODE_BUFS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFF);   // a tile of keys or values has landed
@@ -108,7 +133,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   uint64_t* s_bar = q_bar + 1;                                             // [2] scores complete
   uint64_t* p_bar = s_bar + 2;                                             // [2] weights stored
   uint64_t* o_bar = p_bar + 2;                                             // [2] output complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_bar + 2);
+  uint64_t* code_full = o_bar + 2;                                         // e4m3: codes have landed,
+  uint64_t* code_empty = code_full + CODE_BUFS;                            // have been read,
+  uint64_t* exp_bar = code_empty + CODE_BUFS;                              // [2] the exponents of a key tile are there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exp_bar + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -133,11 +161,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 
   if (tid == 0) {
     for (int i = 0; i < BUFS; ++i) {
-      mbar_init(&full_bar[i], 1);
+      mbar_init(&full_bar[i], Cfg::FP8 ? 4 : 1);
       mbar_init(&empty_bar[i], 1);
+    }
+    for (int i = 0; i < CODE_BUFS; ++i) {
+      mbar_init(&code_full[i], 1);
+      mbar_init(&code_empty[i], 4);
     }
     mbar_init(q_bar, 8);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&exp_bar[i], 4);
       mbar_init(&s_bar[i], 1);
       mbar_init(&p_bar[i], 4);
       mbar_init(&o_bar[i], 1);
@@ -157,7 +190,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   const uint32_t smem_base = smem_u32(smem);
   const int* table = a.page_table + t.seq * a.table_stride;
 
-  if (warp >= 8) {
+  if (warp >= 8 && warp < 12) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::OTHER_REGS));
    if (warp == 9) {
     // ------------------------------ loads ------------------------------
@@ -180,20 +213,29 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       if (page < 0 || page >= a.num_pages) page = (int)a.num_pages;     // past the end: zeros
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        mbar_wait(&empty_bar[buf], phase ^ 1, dead);
-        if (lane == 0) mbar_arrive_expect_tx(&full_bar[buf], Cfg::TILE_BYTES);
-        __syncwarp();
-        if (mine) {
-          const uint32_t dst = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES + lane * box * 128;
+        if constexpr (Cfg::FP8) {
+          mbar_wait(&code_empty[buf], phase ^ 1, dead);
+          if (lane == 0) mbar_arrive_expect_tx(&code_full[buf], Cfg::CODE_BYTES);
+          __syncwarp();
+          const uint32_t dst = smem_base + Cfg::CODE_OFF + buf * Cfg::CODE_BYTES + lane * box * D;
+          if (mine) tma_load_4d(dst, kv ? &tm_v : &tm_k, 0, kvh, place, page, &code_full[buf]);
+          if (++buf == CODE_BUFS) { buf = 0; phase ^= 1; }
+        } else {
+          mbar_wait(&empty_bar[buf], phase ^ 1, dead);
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[buf], Cfg::TILE_BYTES);
+          __syncwarp();
+          if (mine) {
+            const uint32_t dst = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES + lane * box * 128;
 #pragma unroll
-          for (int h = 0; h < Cfg::HALVES; ++h) tma_load_4d(dst + h * 16384, kv ? &tm_v : &tm_k, h * 64, kvh, place, page, &full_bar[buf]);
+            for (int h = 0; h < Cfg::HALVES; ++h) tma_load_4d(dst + h * 16384, kv ? &tm_v : &tm_k, h * 64, kvh, place, page, &full_bar[buf]);
+          }
+          if (++buf == BUFS) { buf = 0; phase ^= 1; }
         }
-        if (++buf == BUFS) { buf = 0; phase ^= 1; }
       }
     }
    } else if (warp == 8) {
     // ------------------------------ MMAs ------------------------------
-    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t fmt = std::is_same<TM, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
     auto scores = [&](int tile, int buf) {            // S[tile] = Q[tile] K^T
@@ -237,9 +279,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     for (int i = 0; i < n_all; ++i) {
       const int vbuf = (2 * i + 1) % BUFS, kbuf = (2 * i + 2) % BUFS;
       landed(2 * i + 1);
-      // Values of tokens that no row sees may be anything, and 0 * NaN is NaN: they become zeros.
+      // Values of tokens that no row sees may be anything, and 0 * NaN is NaN: they become zeros (of an e4m3 cache they
+      // are zeros already).
       const int j0 = (kt0 + i) * 128, from = max(0, lo - j0), to = min(128, hi - j0);
-      if (from > 0 || to < 128) {
+      if (!Cfg::FP8 && (from > 0 || to < 128)) {
         const uint32_t v = smem_base + Cfg::KV_OFF + vbuf * Cfg::TILE_BYTES;
         for (int x = lane; x < 128 * 8 * Cfg::HALVES; x += 32) {      // 16 bytes each
           const int r = (x >> 3) & 127;
@@ -262,6 +305,82 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       if (more) release(kbuf);
     }
    }
+  } else if (warp >= 12) {
+    // ------------------------------ e4m3: codes -> fp16 tiles ------------------------------
+    if constexpr (Cfg::FP8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::OTHER_REGS));
+      const int ct = tid - 384;                       // 0 .. 127: also the token of a key tile whose exponents it fetches
+      constexpr int CH = D / 16;                      // 16-byte pieces of a token's codes
+      constexpr int PASSES = 128 * CH / 128;
+      const int ch = ct % CH, r0 = ct / CH;
+      int kb = 127, vb = 127;
+      auto fetch_exps = [&](int i) {
+        kb = vb = 127;
+        const int j = (kt0 + i) * 128 + ct;
+        if (i >= n_all || j < lo || j >= hi) return;
+        const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+        const int pg = table[p];
+        if (pg < 0 || pg >= a.num_pages) return;
+        const long long at = (long long)pg * a.e_page + (long long)(j - p * a.page_size) * a.e_tok + (long long)kvh * a.e_head;
+        kb = a.key_exp[at];
+        vb = a.value_exp[at];
+      };
+      fetch_exps(0);
+      int buf = 0, cbuf = 0;
+      uint32_t phase = 0, cphase = 0;
+      for (int i = 0; i < n_all; ++i) {
+        const int j0 = (kt0 + i) * 128;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          mbar_wait(&code_full[cbuf], cphase, dead);
+          uint4 w[PASSES];
+          const uint32_t src = smem_base + Cfg::CODE_OFF + cbuf * Cfg::CODE_BYTES + ct * 16;
+#pragma unroll
+          for (int x = 0; x < PASSES; ++x) {
+            w[x] = lds128(src + x * 2048);
+            const int j = j0 + r0 + x * (128 / CH);
+            if (j < lo || j >= hi) w[x] = make_uint4(0, 0, 0, 0);        // tokens that no row sees: anything may lie there
+          }
+          fence_proxy_async();                        // TMA writes the buffer through another proxy than these reads
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&code_empty[cbuf]);
+          if (++cbuf == CODE_BUFS) { cbuf = 0; cphase ^= 1; }
+          mbar_wait(&empty_bar[buf], phase ^ 1, dead);
+          if (kv == 0) {
+            // The buffer was that of the values two key tiles ago: every softmax has read their slot since.
+            float* e = reinterpret_cast<float*>(smem + Cfg::EXP_OFF) + (i & 1) * 384 + ct;
+            e[0] = pow2_of_byte(kb);
+            e[128] = (float)(vb - 127);
+            e[256] = pow2_of_byte(254 - vb);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&exp_bar[i & 1]);
+            fetch_exps(i + 1);
+          }
+          const uint32_t dst = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES;
+#pragma unroll
+          for (int x = 0; x < PASSES; ++x) {
+            const int r = r0 + x * (128 / CH);
+            const uint32_t c4[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+            // Sizes 16 ch .. + 15: two 16-byte pieces of the fp16 row.  Lanes of the second half of a row store them the
+            // other way round, so that a row's lanes meet all eight bank groups.
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int z = y ^ (CH == 8 ? (ch >> 2) : 0);
+              const int piece = 2 * ch + z;
+              const uint32_t lo4 = z ? c4[2] : c4[0], hi4 = z ? c4[3] : c4[1];
+              const uint32_t at = dst + (piece >> 3) * 16384 + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(e4m3x2_to_half2(lo4)), "r"(e4m3x2_hi_to_half2(lo4)),
+                           "r"(e4m3x2_to_half2(hi4)), "r"(e4m3x2_hi_to_half2(hi4))
+                           : "memory");
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full_bar[buf]);
+          if (++buf == BUFS) { buf = 0; phase ^= 1; }
+        }
+      }
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::SOFTMAX_REGS));
     // ------------------------------ softmax: a thread per row ------------------------------
@@ -273,13 +392,33 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     const int qi = rq / a.group, head = kvh * a.group + (rq - qi * a.group);
     const uint32_t qtile = smem_base + Cfg::Q_OFF + tile * Cfg::TILE_BYTES;
     // A negative scale turns the sign of the queries, so that the largest score is the largest product.
-    const float c = fmaxf(fabsf(a.scale_log2), 1e-35f);      // a scale of zero: masked scores stay -inf
+    float c = fmaxf(fabsf(a.scale_log2), 1e-35f);     // a scale of zero: masked scores stay -inf
     {
-      const T* qp = static_cast<const T*>(a.query) + (t.q0 + qi) * a.q_tok + head * a.q_head;
+      const T* qp = static_cast<const T*>(a.query) + (long long)(t.q0 + qi) * a.q_tok + (long long)head * a.q_head;
       const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+      float up = 1.f;
+      if constexpr (!std::is_same<T, TM>::value) {    // bf16 as fp16: see AttnMma
+        float top = 0.f;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          const uint4 w = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
+          const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) top = fmaxf(top, fabsf(Ew<T>::to_f(e[y])));
+        }
+        const int k = attn_row_shift(top);
+        up = __uint_as_float((uint32_t)k << 23);
+        c *= __uint_as_float((uint32_t)(254 - k) << 23);
+      }
 #pragma unroll
       for (int x = 0; x < D / 8; ++x) {
         uint4 w = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
+        if constexpr (!std::is_same<T, TM>::value) {
+          const T* e = reinterpret_cast<const T*>(&w);
+          const uint32_t h[4] = {pack2(Ew<T>::to_f(e[0]) * up, Ew<T>::to_f(e[1]) * up, TM()), pack2(Ew<T>::to_f(e[2]) * up, Ew<T>::to_f(e[3]) * up, TM()),
+                                 pack2(Ew<T>::to_f(e[4]) * up, Ew<T>::to_f(e[5]) * up, TM()), pack2(Ew<T>::to_f(e[6]) * up, Ew<T>::to_f(e[7]) * up, TM())};
+          w = make_uint4(h[0], h[1], h[2], h[3]);
+        }
         const uint32_t at = qtile + (x >> 3) * 16384 + row * 128 + (((x & 7) ^ (row & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x ^ flip), "r"(w.y ^ flip), "r"(w.z ^ flip), "r"(w.w ^ flip)
                      : "memory");
@@ -297,7 +436,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     const int all_lo = a.window > 0 ? base_pos + last_row / a.group - a.window + 1 : 0;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lanes + Cfg::S_COL + tile * 128, o_addr = tmem + lanes + Cfg::O_COL + tile * 128;
-    constexpr float kBias = AttnBias<T>::value / 2;   // weights: at most 2^(8 + 4) in fp16
+    constexpr float kBias = AttnBias<TM>::value / 2;   // weights: at most 2^(8 + 4) in fp16
     float m = -INFINITY, l = 0.f;
 
     // Which of the 16-token groups of a key tile are in the cache (bit g); tokens that no row sees count as there.
@@ -323,6 +462,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
       for (int b = 0; b < 4; ++b) tc_ld32(s_addr + b * 32, v[b]);
       tc_wait_ld();
+      const float* fac = reinterpret_cast<const float*>(smem + Cfg::EXP_OFF) + (i & 1) * 384;
+      if constexpr (Cfg::FP8) {                       // scores -> t_j
+        mbar_wait(&exp_bar[i & 1], (i >> 1) & 1, dead);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            const float4 kf = *reinterpret_cast<const float4*>(fac + b * 32 + x), ev = *reinterpret_cast<const float4*>(fac + 128 + b * 32 + x);
+            const float2 y0 = fma2(mul2(make_float2(__uint_as_float(v[b][x]), __uint_as_float(v[b][x + 1])), make_float2(kf.x, kf.y)),
+                                   make_float2(c, c), make_float2(ev.x, ev.y));
+            const float2 y1 = fma2(mul2(make_float2(__uint_as_float(v[b][x + 2]), __uint_as_float(v[b][x + 3])), make_float2(kf.z, kf.w)),
+                                   make_float2(c, c), make_float2(ev.z, ev.w));
+            v[b][x] = __float_as_uint(y0.x), v[b][x + 1] = __float_as_uint(y0.y);
+            v[b][x + 2] = __float_as_uint(y1.x), v[b][x + 3] = __float_as_uint(y1.y);
+          }
+      }
       if (there != 0xffffffffu || j0 + 128 > all_hi || j0 < all_lo) {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -339,7 +494,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
         for (int x = 1; x < 32; ++x) mx[b] = fmaxf(mx[b], __uint_as_float(v[b][x]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;      // -inf * 0 is NaN, which fmaxf drops
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (Cfg::FP8 ? 1.f : c);
       const float m_new = fmaxf(m, top);
       if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
         if (i > 0) {
@@ -367,12 +522,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
           const int b = h * 2 + (x >> 4), e = (x & 15) * 2;
-          float2 y = fma2(make_float2(__uint_as_float(v[b][e]), __uint_as_float(v[b][e + 1])), c2, off2);
+          const float2 sc = make_float2(__uint_as_float(v[b][e]), __uint_as_float(v[b][e + 1]));
+          float2 y = Cfg::FP8 ? add2(sc, off2) : fma2(sc, c2, off2);
           y.x = exp2_fast(y.x);
           y.y = exp2_fast(y.y);
-          sum.x += y.x;
-          sum.y += y.y;
-          p[x] = pack2(y.x, y.y, T());
+          if constexpr (Cfg::FP8) sum = fma2(y, *reinterpret_cast<const float2*>(fac + 256 + b * 32 + e), sum);
+          else sum = add2(sum, y);
+          p[x] = pack2(y.x, y.y, TM());
         }
         tc_st32(s_addr + h * 32, p);
       }
@@ -431,15 +587,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 }
 
 // The cache as (size, head, place, page), a box = 64 sizes of `box` tokens of one page and head, 128-byte swizzle.
-static bool make_map_cache(CUtensorMap* map, bool bf16, const void* base, const AttnArgs& a, int size, int box) {
+// e4m3: all sizes of the tokens, not swizzled.
+static bool make_map_cache(CUtensorMap* map, CUtensorMapDataType type, const void* base, const AttnArgs& a, int size, int box) {
   auto fn = get_encode_fn();
   if (!fn) return false;
   cuuint64_t dims[4] = {(cuuint64_t)size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.page_size, (cuuint64_t)a.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)a.c_head * 2, (cuuint64_t)a.c_tok * 2, (cuuint64_t)a.c_page * 2};
-  cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1};
+  const bool codes = type == CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const cuuint64_t esz = codes ? 1 : 2;
+  cuuint64_t strides[3] = {a.c_head * esz, a.c_tok * esz, a.c_page * esz};
+  cuuint32_t boxes[4] = {codes ? (cuuint32_t)size : 64, 1, (cuuint32_t)box, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
-            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(map, type, 4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -449,24 +608,25 @@ static int attn_tc_box(int page_size) {
   return box > 128 ? 128 : box;
 }
 
-// Whether the tensor-memory kernel takes the call: a cache of the inputs' type on pages that hold whole groups of 16 tokens.
+// Whether the tensor-memory kernel takes the call: pages that hold whole groups of 16 tokens, strides that TMA takes.
 static bool attn_tc_fits(const AttnArgs& a) {
-  if (a.key_exp != nullptr || a.query_starts == nullptr) return false;
+  if (a.query_starts == nullptr) return false;
   if (attn_tc_box(a.page_size) < 16 || a.num_pages <= 0 || a.num_pages >= 0x7fffffffLL) return false;
   if (a.c_head <= 0 || a.c_tok <= 0 || a.c_page <= 0) return false;
   const long long most = 1LL << 38;                   // strides of a tensor map: below 2^40 bytes
   return a.c_head < most && a.c_tok < most && a.c_page < most;
 }
 
-template <class T, int D>
+template <class T, int D, bool FP8>
 static int launch_attn_tc(const AttnArgs& a, int dev, cudaStream_t st) {
-  using Cfg = AttnTcCfg<D>;
+  using Cfg = AttnTcCfg<D, FP8>;
   static std::atomic<bool> done[64];
   if (!ensure_smem_attr(attn_tc_kernel<T, Cfg>, dev, Cfg::SMEM_ALLOC, done)) return TRB_ERR_CUDA;
   const int box = attn_tc_box(a.page_size);
   CUtensorMap tk, tv;
-  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  if (!make_map_cache(&tk, bf16, a.key_cache, a, D, box) || !make_map_cache(&tv, bf16, a.value_cache, a, D, box)) return TRB_ERR_CUDA;
+  constexpr CUtensorMapDataType type = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                       : std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (!make_map_cache(&tk, type, a.key_cache, a, D, box) || !make_map_cache(&tv, type, a.value_cache, a, D, box)) return TRB_ERR_CUDA;
   const long long per_token = (a.group + 255) / 256;
   long long tiles = (long long)a.tokens * a.group / 256 + a.seqs;
   if (tiles > a.tokens * per_token) tiles = a.tokens * per_token;
