@@ -210,6 +210,29 @@ def test_attention_e4m3_tiny_and_large_values(cuda):
         b.check(b.call())
 
 
+@pytest.mark.parametrize("new", [1, 20, 130])
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("small", [-20, -40])
+def test_attention_to_tiny_values_next_to_large_ones(cuda, new, size, small):
+    """Every third token has values 2^`small` times the others' and all of the weight: the large ones of the same tiles must
+    not take the small ones' bits (bf16 numbers in an e4m3 cache)."""
+    b = Batch(15, [300, 170], [new, new], 8, 2, size, 16, torch.bfloat16, True)
+    for i, n in enumerate(b.lengths):
+        j = torch.arange(n, device="cuda")
+        page, place = b.table[i].long()[j // 16], j % 16
+        tiny = j % 3 == 0
+        e = b.ve[page, place].int()
+        b.ve[page, place] = torch.where(tiny[:, None], e + small, e).to(torch.uint8)
+        keys = b.kc[page, place].float()
+        keys = torch.where(tiny[:, None, None], keys, torch.full_like(keys, -448.0))
+        b.kc.view(torch.uint8)[page, place] = keys.to(torch.float8_e4m3fn).view(torch.uint8)
+    b.q = b.q.abs() + 0.25
+    b.check(b.call())
+    k, v = b.tokens(0)
+    o, _, _ = plain_attention(b.q[:new], k, v, 300, new, size ** -0.5, True, None)
+    assert float(o.abs().max()) < 2.0 ** -16       # against values of about 1: the case is what it says
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("plan", [DECODE, CHUNKS, LONG], ids=["decode", "chunks", "long"])
 def test_attention_strides(cuda, e4m3, plan):

@@ -41,9 +41,12 @@ struct AttnTcCfg {
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int CODE_OFF = KV_OFF + BUFS * TILE_BYTES;
-  static constexpr int EXP_OFF = CODE_OFF + CODE_BUFS * CODE_BYTES;      // float [2][3][128]: 2^e of keys; e and 2^-e of values
-  static constexpr int BAR_OFF = EXP_OFF + (FP8 ? 2 * 3 * 128 * 4 : 0);
-  static constexpr int NUM_BARS = 2 * BUFS + 1 + 3 * 2 + 2 * CODE_BUFS + 2;
+  // e4m3, per key tile modulo 2: 2^E of the keys, E of the values, 2^-E, whether values have rests, the rests [128].
+  static constexpr int EXP_OFF = CODE_OFF + CODE_BUFS * CODE_BYTES, EXP_FLOATS = 4 + 128;
+  static constexpr int SCALE_OFF = EXP_OFF + (FP8 ? 2 * EXP_FLOATS * 4 : 0);      // fp16 [2][2][128]: factors of keys and values
+  static constexpr int MAX_OFF = SCALE_OFF + (FP8 ? 2 * 2 * 128 * 2 : 0);         // int [2][2][2]: two warps' largest exponents
+  static constexpr int BAR_OFF = MAX_OFF + (FP8 ? 32 : 0);
+  static constexpr int NUM_BARS = 2 * BUFS + 1 + 4 * 2 + 2 * CODE_BUFS + 6;
   static constexpr int SMEM_BYTES = BAR_OFF + NUM_BARS * 8 + 16;
   static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;
   static constexpr int GROUPS = FP8 ? 4 : 3;             // warpgroups
@@ -63,25 +66,46 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tc_commit_one(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The issuing instructions below carry the elected lane as a predicate: the warp stays converged around them.
+__device__ __forceinline__ void tc_commit_one(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(elected)
+      : "memory");
 }
 // D[128, N] (+)= A[128, 16] B[16, N]; A and B in shared memory.
-__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                              uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
       : "memory");
 }
 // The same with A in tensor memory: 8 columns of two 16-bit numbers per row.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                              uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+// Waits for the warp's loads from tensor memory; the registers pass through, so that no use of them moves before it.
+__device__ __forceinline__ void tc_wait_ld32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+      "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -119,6 +143,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <class T, class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a, int tiles_bound,
@@ -131,12 +161,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   uint64_t* empty_bar = full_bar + BUFS;                                   // its MMAs have retired
   uint64_t* q_bar = empty_bar + BUFS;                                      // the queries are in shared memory
   uint64_t* s_bar = q_bar + 1;                                             // [2] scores complete
-  uint64_t* p_bar = s_bar + 2;                                             // [2] weights stored
-  uint64_t* o_bar = p_bar + 2;                                             // [2] output complete
+  uint64_t* p_bar = s_bar + 2;                                             // [2][2] weights of the first and the last 64 keys stored
+  uint64_t* o_bar = p_bar + 4;                                             // [2] output complete
   uint64_t* code_full = o_bar + 2;                                         // e4m3: codes have landed,
   uint64_t* code_empty = code_full + CODE_BUFS;                            // have been read,
   uint64_t* exp_bar = code_empty + CODE_BUFS;                              // [2] the exponents of a key tile are there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exp_bar + 2);
+  uint64_t* fac_bar = exp_bar + 2;                                         // [2] its factors are there,
+  uint64_t* fac_free = fac_bar + 2;                                        // [2] both have been read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fac_free + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -155,7 +187,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     const int rows = min(128, t.rows - 128 * i);
     int h = hi;
     if (a.causal && rows > 0) h = min(hi, base_pos + (t.row0 + 128 * i + rows - 1) / a.group + 1);
-    n[i] = rows > 0 && h > lo ? (h + 127) / 128 - kt0 : 0;
+    // The same in every lane, which the reduction tells the compiler: loop counters and the MMAs' operands stay in uniform
+    // registers.
+    n[i] = __reduce_max_sync(0xffffffffu, rows > 0 && h > lo ? (h + 127) / 128 - kt0 : 0);
   }
   const int n_all = max(n[0], n[1]);
 
@@ -170,9 +204,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     }
     mbar_init(q_bar, 8);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&exp_bar[i], 4);
+      mbar_init(&exp_bar[i], 2);
+      mbar_init(&fac_bar[i], 2);
+      mbar_init(&fac_free[i], 4 + 8);
       mbar_init(&s_bar[i], 1);
-      mbar_init(&p_bar[i], 4);
+      mbar_init(&p_bar[2 * i], 4);
+      mbar_init(&p_bar[2 * i + 1], 4);
       mbar_init(&o_bar[i], 1);
     }
     *dead = 0;
@@ -186,7 +223,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot);
   const uint32_t smem_base = smem_u32(smem);
   const int* table = a.page_table + t.seq * a.table_stride;
 
@@ -241,29 +278,33 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     auto scores = [&](int tile, int buf) {            // S[tile] = Q[tile] K^T
       const uint64_t qd = tc_smem_desc(smem_base + Cfg::Q_OFF + tile * Cfg::TILE_BYTES);
       const uint64_t kd = tc_smem_desc(smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES);
-      if (elect_one()) {
+      const uint32_t one = elect_one();
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {            // 32 bytes along a row; the next 64 sizes are 16 KB further
-          const uint64_t step = (uint64_t)((k >> 2) * (16384 >> 4) + (k & 3) * 2);
-          tc_mma_f16_ss(tmem + Cfg::S_COL + tile * 128, qd + step, kd + step, idesc_s, k > 0);
-        }
-        tc_commit_one(&s_bar[tile]);
+      for (int k = 0; k < D / 16; ++k) {              // 32 bytes along a row; the next 64 sizes are 16 KB further
+        const uint64_t step = (uint64_t)((k >> 2) * (16384 >> 4) + (k & 3) * 2);
+        tc_mma_f16_ss(tmem + Cfg::S_COL + tile * 128, qd + step, kd + step, idesc_s, k > 0, one);
       }
+      tc_commit_one(&s_bar[tile], one);
       __syncwarp();
     };
-    auto outputs = [&](int tile, int buf, bool first, bool last) {      // O[tile] += P[tile] V
+    // O[tile] += P[tile] V, 64 keys as soon as their weights are there.
+    auto outputs = [&](int tile, int buf, int i) {
       const uint32_t v = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES;
-      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)                   // 16 tokens = 16 rows of 128 bytes
-          tc_mma_f16_ts(tmem + Cfg::O_COL + tile * 128, tmem + Cfg::S_COL + tile * 128 + k * 8,
-                        tc_smem_desc_mn(v + k * 2048, 16384, 1024), idesc_o, !first || k > 0);
-        if (last) tc_commit_one(&o_bar[tile]);
+      for (int h = 0; h < 2; ++h) {
+        mbar_wait(&p_bar[2 * tile + h], i & 1, dead);
+        tc_fence_after();
+        const uint32_t one = elect_one();
+#pragma unroll
+        for (int k = 4 * h; k < 4 * h + 4; ++k)       // 16 tokens = 16 rows of 128 bytes
+          tc_mma_f16_ts(tmem + Cfg::O_COL + tile * 128, tmem + Cfg::S_COL + tile * 128 + k * 8, tc_smem_desc_mn(v + k * 2048, 16384, 1024),
+                        idesc_o, i > 0 || k > 0, one);
+        if (h == 1 && i + 1 == n[tile]) tc_commit_one(&o_bar[tile], one);
+        __syncwarp();
       }
-      __syncwarp();
     };
     auto release = [&](int buf) {
-      if (elect_one()) tc_commit_one(&empty_bar[buf]);
+      tc_commit_one(&empty_bar[buf], elect_one());
       __syncwarp();
     };
     // Items of the ring: K of key tile i is number 2i, V number 2i + 1.
@@ -293,47 +334,107 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       }
       const bool more = i + 1 < n_all;
       for (int tile = 0; tile < 2; ++tile) {
-        if (i < n[tile]) {
-          mbar_wait(&p_bar[tile], i & 1, dead);
-          tc_fence_after();
-          outputs(tile, vbuf, i == 0, i + 1 == n[tile]);
-        }
+        if (i < n[tile]) outputs(tile, vbuf, i);
         if (more && tile == 0) landed(2 * i + 2);
         if (i + 1 < n[tile]) scores(tile, kbuf);
       }
       release(vbuf);
       if (more) release(kbuf);
     }
+   } else if (Cfg::FP8) {
+    // ------------------------------ e4m3: exponents and factors (warps 10, 11) ------------------------------
+    // A lane has two tokens of a key tile.  Page numbers are asked for two tiles ahead and exponents one, so that neither load
+    // is waited for.
+    const int first = (warp - 10) * 32 + lane;
+    int page[2], place[2], kb[2], vb[2];              // of the next tile but one; of the next tile (-1: not there)
+    auto ask_pages = [&](int i) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = (kt0 + i) * 128 + first + 64 * x;
+        page[x] = -1;
+        place[x] = 0;
+        if (i < n_all && j >= lo && j < hi) {
+          const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+          page[x] = table[p];
+          place[x] = j - p * a.page_size;
+        }
+      }
+    };
+    auto ask_exps = [&]() {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        kb[x] = vb[x] = -1;
+        if (page[x] >= 0 && page[x] < a.num_pages) {
+          const long long at = (long long)page[x] * a.e_page + (long long)place[x] * a.e_tok + (long long)kvh * a.e_head;
+          kb[x] = a.key_exp[at];
+          vb[x] = a.value_exp[at];
+        }
+      }
+    };
+    int2* maxima = reinterpret_cast<int2*>(smem + Cfg::MAX_OFF);
+    ask_pages(0);
+    ask_exps();
+    ask_pages(1);
+    for (int i = 0; i < n_all; ++i) {
+      const int s = i & 1;
+      // The slot is free once the converting warps have its factors and every softmax that uses the tile its exponents.
+      mbar_wait(&fac_free[s], ((i >> 1) & 1) ^ 1, dead);
+      const int2 most = make_int2(__reduce_max_sync(0xffffffffu, max(kb[0], kb[1])), __reduce_max_sync(0xffffffffu, max(vb[0], vb[1])));
+      if (lane == 0) maxima[2 * s + (warp - 10)] = most;
+      named_bar_sync(1, 64);
+      const int2 m0 = maxima[2 * s], m1 = maxima[2 * s + 1];
+      int ek = max(m0.x, m1.x), ev = max(m0.y, m1.y);
+      if (ek < 0) ek = ev = 127;                      // no token of the tile is there
+      float* e = reinterpret_cast<float*>(smem + Cfg::EXP_OFF) + s * Cfg::EXP_FLOATS;
+      __half* scales = reinterpret_cast<__half*>(smem + Cfg::SCALE_OFF) + s * 256;
+      bool any = false;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int tok = first + 64 * x;
+        const int kd = ek - kb[x], vd = min(ev - vb[x], 15);
+        const float rest = vb[x] >= 0 ? (float)(vb[x] + vd - ev) : 0.f;
+        scales[tok] = kd > 24 ? __float2half_rn(0.f) : __float2half_rn(pow2_of_byte(127 - kd));
+        scales[128 + tok] = __float2half_rn(pow2_of_byte(127 - vd));
+        e[4 + tok] = rest;
+        any |= rest != 0.f;
+      }
+      any = __any_sync(0xffffffffu, any);
+      if (lane == 0) reinterpret_cast<uint16_t*>(e + 3)[warp - 10] = any ? 1 : 0;      // two halves, read as one number
+      if (tid == 320) {
+        e[0] = pow2_of_byte(ek);
+        e[1] = (float)(ev - 127);
+        e[2] = pow2_of_byte(254 - ev);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&fac_bar[s]);
+        mbar_arrive(&exp_bar[s]);
+      }
+      ask_exps();
+      ask_pages(i + 2);
+    }
    }
   } else if (warp >= 12) {
     // ------------------------------ e4m3: codes -> fp16 tiles ------------------------------
     if constexpr (Cfg::FP8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::OTHER_REGS));
-      const int ct = tid - 384;                       // 0 .. 127: also the token of a key tile whose exponents it fetches
+      const int ct = tid - 384;                       // 0 .. 127
       constexpr int CH = D / 16;                      // 16-byte pieces of a token's codes
       constexpr int PASSES = 128 * CH / 128;
       const int ch = ct % CH, r0 = ct / CH;
-      int kb = 127, vb = 127;
-      auto fetch_exps = [&](int i) {
-        kb = vb = 127;
-        const int j = (kt0 + i) * 128 + ct;
-        if (i >= n_all || j < lo || j >= hi) return;
-        const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-        const int pg = table[p];
-        if (pg < 0 || pg >= a.num_pages) return;
-        const long long at = (long long)pg * a.e_page + (long long)(j - p * a.page_size) * a.e_tok + (long long)kvh * a.e_head;
-        kb = a.key_exp[at];
-        vb = a.value_exp[at];
-      };
-      fetch_exps(0);
       int buf = 0, cbuf = 0;
       uint32_t phase = 0, cphase = 0;
       for (int i = 0; i < n_all; ++i) {
         const int j0 = (kt0 + i) * 128;
+        mbar_wait(&fac_bar[i & 1], (i >> 1) & 1, dead);
+        const __half* scales = reinterpret_cast<const __half*>(smem + Cfg::SCALE_OFF) + (i & 1) * 256;
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           mbar_wait(&code_full[cbuf], cphase, dead);
           uint4 w[PASSES];
+          __half2 f[PASSES];
+#pragma unroll
+          for (int x = 0; x < PASSES; ++x) f[x] = __half2half2(scales[kv * 128 + r0 + x * (128 / CH)]);
           const uint32_t src = smem_base + Cfg::CODE_OFF + cbuf * Cfg::CODE_BYTES + ct * 16;
 #pragma unroll
           for (int x = 0; x < PASSES; ++x) {
@@ -346,20 +447,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           if (lane == 0) mbar_arrive(&code_empty[cbuf]);
           if (++cbuf == CODE_BUFS) { cbuf = 0; cphase ^= 1; }
           mbar_wait(&empty_bar[buf], phase ^ 1, dead);
-          if (kv == 0) {
-            // The buffer was that of the values two key tiles ago: every softmax has read their slot since.
-            float* e = reinterpret_cast<float*>(smem + Cfg::EXP_OFF) + (i & 1) * 384 + ct;
-            e[0] = pow2_of_byte(kb);
-            e[128] = (float)(vb - 127);
-            e[256] = pow2_of_byte(254 - vb);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&exp_bar[i & 1]);
-            fetch_exps(i + 1);
-          }
           const uint32_t dst = smem_base + Cfg::KV_OFF + buf * Cfg::TILE_BYTES;
 #pragma unroll
           for (int x = 0; x < PASSES; ++x) {
             const int r = r0 + x * (128 / CH);
+            auto times = [&](uint32_t h) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h), f[x]);
+              return *reinterpret_cast<const uint32_t*>(&y);
+            };
             const uint32_t c4[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
             // Sizes 16 ch .. + 15: two 16-byte pieces of the fp16 row.  Lanes of the second half of a row store them the
             // other way round, so that a row's lanes meet all eight bank groups.
@@ -369,8 +464,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
               const int piece = 2 * ch + z;
               const uint32_t lo4 = z ? c4[2] : c4[0], hi4 = z ? c4[3] : c4[1];
               const uint32_t at = dst + (piece >> 3) * 16384 + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(e4m3x2_to_half2(lo4)), "r"(e4m3x2_hi_to_half2(lo4)),
-                           "r"(e4m3x2_to_half2(hi4)), "r"(e4m3x2_hi_to_half2(hi4))
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(times(e4m3x2_to_half2(lo4))),
+                           "r"(times(e4m3x2_hi_to_half2(lo4))), "r"(times(e4m3x2_to_half2(hi4))), "r"(times(e4m3x2_hi_to_half2(hi4)))
                            : "memory");
             }
           }
@@ -379,6 +474,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           if (lane == 0) mbar_arrive(&full_bar[buf]);
           if (++buf == BUFS) { buf = 0; phase ^= 1; }
         }
+        if (lane == 0) mbar_arrive(&fac_free[i & 1]);
       }
     }
   } else {
@@ -439,62 +535,98 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     constexpr float kBias = AttnBias<TM>::value / 2;   // weights: at most 2^(8 + 4) in fp16
     float m = -INFINITY, l = 0.f;
 
-    // Which of the 16-token groups of a key tile are in the cache (bit g); tokens that no row sees count as there.
-    auto groups_there = [&](int i) -> uint32_t {
-      bool there = true;
-      if (lane < 8) {
-        const int j = (kt0 + i) * 128 + lane * 16;
-        if (j < hi && j + 16 > lo) {
-          const int pg = table[a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size];
-          there = pg >= 0 && pg < a.num_pages;
-        }
-      }
-      return __ballot_sync(0xffffffffu, there);
+    // Page of this lane's 16-token group of key tile i (lanes 0-7); 0 for tokens that no row sees.  Asked for a tile ahead and
+    // looked at only then: the load would otherwise stand in the loop (600 of 3400 clocks a tile).
+    auto page_of = [&](int i) -> int {
+      const int j = (kt0 + i) * 128 + lane * 16;
+      if (lane >= 8 || i >= n[tile] || j >= hi || j + 16 <= lo) return 0;
+      return table[a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size];
     };
-    uint32_t there_next = n[tile] > 0 ? groups_there(0) : 0u;
+    int page = page_of(0);
     for (int i = 0; i < n[tile]; ++i) {
-      const uint32_t there = there_next;
-      if (i + 1 < n[tile]) there_next = groups_there(i + 1);
+      // Which of the groups are in the cache (bit g).
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);
+      page = page_of(i + 1);
       const int j0 = (kt0 + i) * 128;
       mbar_wait(&s_bar[tile], i & 1, dead);
       tc_fence_after();
-      uint32_t v[4][32];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) tc_ld32(s_addr + b * 32, v[b]);
-      tc_wait_ld();
-      const float* fac = reinterpret_cast<const float*>(smem + Cfg::EXP_OFF) + (i & 1) * 384;
-      if constexpr (Cfg::FP8) {                       // scores -> t_j
+      // e4m3: the tile's codes carry 2^(e_j - E) already, E the largest exponent of the tile (one for keys, one for values);
+      // values further than 2^15 below the largest of their tile would leave fp16 and keep a rest, which enters per token.
+      float ct = c, add = 0.f, back = 1.f;
+      const float* fac = nullptr;
+      bool rests = false;
+      if constexpr (Cfg::FP8) {
         mbar_wait(&exp_bar[i & 1], (i >> 1) & 1, dead);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            const float4 kf = *reinterpret_cast<const float4*>(fac + b * 32 + x), ev = *reinterpret_cast<const float4*>(fac + 128 + b * 32 + x);
-            const float2 y0 = fma2(mul2(make_float2(__uint_as_float(v[b][x]), __uint_as_float(v[b][x + 1])), make_float2(kf.x, kf.y)),
-                                   make_float2(c, c), make_float2(ev.x, ev.y));
-            const float2 y1 = fma2(mul2(make_float2(__uint_as_float(v[b][x + 2]), __uint_as_float(v[b][x + 3])), make_float2(kf.z, kf.w)),
-                                   make_float2(c, c), make_float2(ev.z, ev.w));
-            v[b][x] = __float_as_uint(y0.x), v[b][x + 1] = __float_as_uint(y0.y);
-            v[b][x + 2] = __float_as_uint(y1.x), v[b][x + 3] = __float_as_uint(y1.y);
-          }
+        fac = reinterpret_cast<const float*>(smem + Cfg::EXP_OFF) + (i & 1) * Cfg::EXP_FLOATS;
+        ct = fmaxf(c * fac[0], 1e-35f);               // never zero: masked scores stay -inf
+        add = fac[1];
+        back = fac[2];
+        rests = reinterpret_cast<const int*>(fac)[3] != 0;
       }
-      if (there != 0xffffffffu || j0 + 128 > all_hi || j0 < all_lo) {
+      const float cs = rests ? 1.f : ct;
+      const bool masked = there != 0xffffffffu || j0 + 128 > all_hi || j0 < all_lo;
+      // Bit x: this row sees token j0 + 32 b + x.
+      auto seen = [&](int b) -> uint32_t {
+        const int h = row_hi - j0 - 32 * b, lw = row_lo - j0 - 32 * b;
+        uint32_t bits = h >= 32 ? 0xffffffffu : h <= 0 ? 0u : (1u << h) - 1u;
+        bits &= lw <= 0 ? 0xffffffffu : lw >= 32 ? 0u : ~((1u << lw) - 1u);
+        return bits & (((there >> (2 * b)) & 1 ? 0xffffu : 0u) | ((there >> (2 * b + 1)) & 1 ? 0xffff0000u : 0u));
+      };
+      auto mask = [&](uint32_t (&w)[32], uint32_t bits) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int x = 0; x < 32; ++x) w[x] = (bits >> x) & 1 ? w[x] : 0xff800000u;      // -inf
+      };
+      // e4m3: masks and rests are rare and go through tensor memory, which keeps them out of the loops below.
+      if (Cfg::FP8 && (masked || rests)) {
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          uint32_t w[32];
+          tc_ld32(s_addr + b * 32, w);
+          tc_wait_ld32(w);
+          if (rests) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int j = j0 + b * 32 + x;
-            if (j >= row_hi || j < row_lo || !((there >> (b * 2 + (x >> 4))) & 1)) v[b][x] = 0xff800000u;   // -inf
+            for (int x = 0; x < 32; ++x) w[x] = __float_as_uint(fmaf(__uint_as_float(w[x]), ct, fac[4 + b * 32 + x]));
           }
+          mask(w, seen(b));
+          tc_st32(s_addr + b * 32, w);
+        }
+        tc_wait_st();
       }
-      float mx[4];
+      // The whole row in registers; e4m3, where four more warps need some: read twice, 32 scores at a time and the next 32 on
+      // their way, once for the maximum and once for the weights (a row held there spills; the other way round, a second
+      // reading costs 4%: 8192-token prompt 551 -> 577 us).
+      constexpr int HELD = Cfg::FP8 ? 2 : 4;
+      uint32_t v[HELD][32];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < HELD - 1; ++b) tc_ld32(s_addr + b * 32, v[b]);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        mx[b] = __uint_as_float(v[b][0]);
+        uint32_t (&w)[32] = v[b % HELD];
+        if (Cfg::FP8) {
+          tc_wait_ld32(w);
+          if (b < 3) tc_ld32(s_addr + (b + 1) * 32, v[(b + 1) % HELD]);
+        } else if (b == 0) {
+          tc_ld32(s_addr + 96, v[HELD - 1]);
 #pragma unroll
-        for (int x = 1; x < 32; ++x) mx[b] = fmaxf(mx[b], __uint_as_float(v[b][x]));
+          for (int x = 0; x < HELD; ++x) tc_wait_ld32(v[x]);
+          if (masked) {
+#pragma unroll
+            for (int x = 0; x < HELD; ++x) mask(v[x], seen(x));
+          }
+        }
+        float m4[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) m4[x] = max3(__uint_as_float(w[x]), __uint_as_float(w[x + 4]), __uint_as_float(w[x + 8]));
+#pragma unroll
+        for (int x = 12; x < 28; x += 8)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) m4[y] = max3(m4[y], __uint_as_float(w[x + y]), __uint_as_float(w[x + 4 + y]));
+#pragma unroll
+        for (int y = 0; y < 4; ++y) mx = max3(mx, m4[y], __uint_as_float(w[28 + y]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (Cfg::FP8 ? 1.f : c);
+      if (Cfg::FP8) tc_ld32(s_addr, v[0]);
+      const float top = fmaf(mx, cs, add);
       const float m_new = fmaxf(m, top);
       if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
         if (i > 0) {
@@ -505,7 +637,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           for (int b = 0; b < D / 32; ++b) {
             uint32_t o[32];
             tc_ld32(o_addr + b * 32, o);
-            tc_wait_ld();
+            tc_wait_ld32(o);
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
             tc_st32(o_addr + b * 32, o);
@@ -513,30 +645,53 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         m = m_new;
       }
-      const float off = kBias - (m == -INFINITY ? 0.f : m);
-      const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+      const float off = kBias + add - (m == -INFINITY ? 0.f : m);
+      const float2 c2 = make_float2(cs, cs), off2 = make_float2(off, off);
       float2 sum = make_float2(0.f, 0.f);
+      float rest_sum = 0.f;                           // of the weights without the values' rests
+      if (Cfg::FP8 && rests) {
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          uint32_t w[32];
+          tc_ld32(s_addr + b * 32, w);
+          tc_wait_ld32(w);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
+          for (int x = 0; x < 32; ++x) rest_sum += exp2_fast(__uint_as_float(w[x]) + off - fac[4 + b * 32 + x]);
+        }
+      }
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const int b = h * 2 + (x >> 4), e = (x & 15) * 2;
-          const float2 sc = make_float2(__uint_as_float(v[b][e]), __uint_as_float(v[b][e + 1]));
-          float2 y = Cfg::FP8 ? add2(sc, off2) : fma2(sc, c2, off2);
+      for (int b = 0; b < 4; ++b) {
+        uint32_t (&w)[32] = v[b % HELD];
+        if (Cfg::FP8) {
+          tc_wait_ld32(w);
+          if (b < 3) tc_ld32(s_addr + (b + 1) * 32, v[(b + 1) % HELD]);
+        }
+        uint32_t p[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float2 sc = make_float2(__uint_as_float(w[2 * x]), __uint_as_float(w[2 * x + 1]));
+          float2 y = fma2(sc, c2, off2);
           y.x = exp2_fast(y.x);
           y.y = exp2_fast(y.y);
-          if constexpr (Cfg::FP8) sum = fma2(y, *reinterpret_cast<const float2*>(fac + 256 + b * 32 + e), sum);
-          else sum = add2(sum, y);
+          sum = add2(sum, y);
           p[x] = pack2(y.x, y.y, TM());
         }
-        tc_st32(s_addr + h * 32, p);
+        tc_st16(s_addr + b * 16, p);                  // over scores that have been read
+        if (b & 1) {
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_bar[2 * tile + (b >> 1)]);
+        }
       }
-      l += sum.x + sum.y;
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_bar[tile]);
+      l = fmaf(rests ? rest_sum : sum.x + sum.y, back, l);
+      if (Cfg::FP8 && lane == 0) mbar_arrive(&fac_free[i & 1]);
+    }
+    if (Cfg::FP8) {                                   // the other tile's last key tiles: this one has no use for them
+      for (int i = n[tile]; i < n_all; ++i) {
+        mbar_wait(&exp_bar[i & 1], (i >> 1) & 1, dead);
+        if (lane == 0) mbar_arrive(&fac_free[i & 1]);
+      }
     }
     // ------------------------------ epilogue ------------------------------
     if (n[tile] > 0) {
@@ -553,7 +708,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       uint32_t o[32] = {};
       if (n[tile] > 0) {
         tc_ld32(o_addr + b * 32, o);
-        tc_wait_ld();
+        tc_wait_ld32(o);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
