@@ -356,7 +356,8 @@ def test_attention_far_into_a_document(cuda, e4m3):
 # ------------------------------------------------------------------------------------------------ cache
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("quantised", [False, True])
-@pytest.mark.parametrize("T,heads,size,page", [(1, 1, 128, 16), (7, 8, 64, 16), (333, 5, 80, 24), (61, 40, 128, 1), (19, 2, 256, 128), (2000, 3, 8, 32)])
+@pytest.mark.parametrize("T,heads,size,page", [(1, 1, 128, 16), (7, 8, 64, 16), (333, 5, 80, 24), (61, 40, 128, 1), (19, 2, 256, 128), (2000, 3, 8, 32), (5, 150, 32, 16),
+                                                    (3, 700, 8, 16), (700, 33, 16, 16)])
 def test_cache_write_and_read(cuda, dtype, quantised, T, heads, size, page):
     g = gen(20)
     pages = -(-T // page) + 2

@@ -576,8 +576,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
         for (int x = 0; x < 32; ++x) w[x] = (bits >> x) & 1 ? w[x] : 0xff800000u;      // -inf
       };
-      // e4m3: masks and rests are rare and go through tensor memory, which keeps them out of the loops below.
-      if (Cfg::FP8 && (masked || rests)) {
+      // Masks and rests are rare and go through tensor memory, which keeps their code out of the loops below: with it the
+      // loops ran out of the instruction cache (e4m3, two chunks over 12000 tokens: 467 us, without 311).
+      if (masked || rests) {
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
           uint32_t w[32];
@@ -610,10 +611,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           tc_ld32(s_addr + 96, v[HELD - 1]);
 #pragma unroll
           for (int x = 0; x < HELD; ++x) tc_wait_ld32(v[x]);
-          if (masked) {
-#pragma unroll
-            for (int x = 0; x < HELD; ++x) mask(v[x], seen(x));
-          }
         }
         float m4[4];
 #pragma unroll

@@ -4,9 +4,10 @@
 //   r = 1 / sqrt(mean_d x_d^2 + eps),  y_d = x_d r w_d,  first rot_dim elements of y: (a, b) -> (a c - b s, b c + a s)
 // for the pairs (i, i + rot_dim / 2) (NeoX) or (2i, 2i + 1) (GPT-J).  32-bit arithmetic, one rounding at the end.
 //
-// A group of G = head_size / 8 lanes (rounded up to a power of two) holds one head, 8 elements = 16 bytes a lane:
-// the sum of squares is log2(G) shuffles, a NeoX partner is one shuffle per element away.  A group goes through
-// several heads of ONE token, so the token's cosines and sines and the weights are read once and stay in registers.
+// A group of G = head_size / 8 lanes (rounded up to a power of two) holds one head, 8 elements = 16 bytes a lane: the sum of
+// squares is log2(G) shuffles, a NeoX partner's inputs come with four more.  A group has up to five heads of ONE token and
+// asks for all of them, for the position and then for its cosines and sines at once, so that a CTA waits for memory twice and
+// no more: with loops over the heads of a token (fewer and longer CTAs) 8191 x 80 heads took 80 to 90 us, now 61 (5.5 TB/s; four heads a group 74, eight 74).
 #pragma once
 
 #include "elementwise.cuh"
@@ -39,123 +40,158 @@ struct QkNormArgs {
 };
 
 constexpr int kQkThreads = 128;
-enum RotMode { kNeoxLanes, kNeoxAny, kPairs };   // NeoX with rot_dim / 2 a multiple of 8, any other NeoX, GPT-J
+constexpr int kQkHeads = 5;           // heads of a group, all loaded together
+// NeoX and GPT-J; "Any": rot_dim / 2 is no multiple of 8 (4), or the table or the weights are not 16-byte aligned, so that
+// cosines, sines and weights come one by one (and a NeoX partner through shared memory).
+enum RotMode { kNeox, kNeoxAny, kPairs, kPairsAny };
 
 __device__ __forceinline__ float table_value(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float table_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float table_value(const float* p) { return *p; }
 
+// N numbers from an aligned address.
+template <int N, class TC>
+__device__ __forceinline__ void table_values(const TC* p, float* v) {
+  constexpr int BYTES = N * (int)sizeof(TC), PIECE = BYTES < 16 ? 8 : 16;
+  using Word = typename std::conditional<PIECE == 16, uint4, uint2>::type;
+#pragma unroll
+  for (int i = 0; i < BYTES / PIECE; ++i) {
+    const Word w = reinterpret_cast<const Word*>(p)[i];
+#pragma unroll
+    for (int e = 0; e < PIECE / (int)sizeof(TC); ++e) v[i * (PIECE / (int)sizeof(TC)) + e] = table_value(reinterpret_cast<const TC*>(&w) + e);
+  }
+}
+
 template <class T, class TC, int G, int MODE>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNormArgs a) {
   constexpr int GROUPS = kQkThreads / G;
-  constexpr int AHEAD = 4;            // heads whose loads are in flight together
-  __shared__ float swap[MODE == kNeoxAny ? GROUPS : 1][MODE == kNeoxAny ? G * 8 : 1];
+  constexpr bool PAIRS = MODE == kPairs || MODE == kPairsAny;
+  __shared__ uint4 swap[MODE == kNeoxAny ? GROUPS : 1][MODE == kNeoxAny ? G : 1];
   const long long t = blockIdx.x;
   const int li = threadIdx.x % G, grp = threadIdx.x / G;
   const int d0 = li * 8;              // first of this lane's elements
   const bool active = d0 < a.head_size;
+  const bool is_key = blockIdx.z != 0;
+  const int heads = is_key ? a.num_kv_heads : a.num_heads;
+  const int step = gridDim.y * GROUPS, h0 = blockIdx.y * GROUPS + grp;
+  if (h0 >= heads) return;
+  const T* in = is_key ? static_cast<const T*>(a.key) + t * a.k_stride : static_cast<const T*>(a.query) + t * a.q_stride;
+  T* out = is_key ? static_cast<T*>(a.key_out) + t * a.ko_stride : static_cast<T*>(a.query_out) + t * a.qo_stride;
+  uint4 raw[kQkHeads];                // all loads in flight, before the position is known
+#pragma unroll
+  for (int u = 0; u < kQkHeads; ++u) {
+    const int h = h0 + u * step;
+    raw[u] = make_uint4(0, 0, 0, 0);
+    if (active && h < heads) raw[u] = *reinterpret_cast<const uint4*>(in + (long long)h * a.head_size + d0);
+  }
   const int64_t pos = a.positions[t];
-  if (pos < 0 || pos >= a.max_position) return;     // a padding token
+  const T* w = static_cast<const T*>(is_key ? a.key_weight : a.query_weight);
   const int half = a.rot_dim / 2;
-  const TC* row = static_cast<const TC*>(a.table) + pos * a.rot_dim;
-  float c[8], s[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int d = d0 + e;
-    const bool turn = d < a.rot_dim;
-    const int i = !turn ? 0 : MODE == kPairs ? d >> 1 : d < half ? d : d - half;
-    c[e] = turn ? table_value(row + i) : 1.f;
-    const float sn = turn ? table_value(row + half + i) : 0.f;
-    s[e] = (MODE == kPairs ? (d & 1) == 0 : d < half) ? -sn : sn;   // the sign that goes with the partner
-  }
-  const int total = a.num_heads + a.num_kv_heads;
-  const int step = gridDim.y * GROUPS;
   const unsigned lanes = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << ((threadIdx.x & 31) / G * G);
-  float wq[8], wk[8];
+  // y_d = r (x_d own_d + x_partner other_d): own = weight x cosine, other = the partner's weight x sine with its sign.
+  float own[8], other[8];
+  const bool there = pos >= 0 && pos < a.max_position;        // not: a padding token
+  const TC* row = static_cast<const TC*>(a.table) + (there ? pos : 0) * a.rot_dim;
+  if constexpr (MODE == kNeox || MODE == kPairs) {
+    // A lane's eight elements turn together or not at all.
+    const bool turn = there && d0 < a.rot_dim;
+    const int i = !turn ? 0 : PAIRS ? d0 >> 1 : d0 < half ? d0 : d0 - half;
+    const int partner = !turn || PAIRS ? d0 : d0 < half ? d0 + half : d0 - half;
+    float c[8], sn[8], ww[8], wp[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = active && a.query_weight ? Ew<T>::to_f(static_cast<const T*>(a.query_weight)[d0 + e]) : 1.f;
-    wk[e] = active && a.key_weight ? Ew<T>::to_f(static_cast<const T*>(a.key_weight)[d0 + e]) : 1.f;
-  }
-  for (int h0 = blockIdx.y * GROUPS + grp; h0 < total; h0 += AHEAD * step) {
-    uint4 raw[AHEAD];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int h = h0 + u * step;
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (active && h < total) {
-        const T* p = h < a.num_heads ? static_cast<const T*>(a.query) + t * a.q_stride + (long long)h * a.head_size
-                                     : static_cast<const T*>(a.key) + t * a.k_stride + (long long)(h - a.num_heads) * a.head_size;
-        raw[u] = *reinterpret_cast<const uint4*>(p + d0);
-      }
+    for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f, ww[e] = wp[e] = 1.f;
+    if (turn) {
+      table_values<PAIRS ? 4 : 8>(row + i, c);
+      table_values<PAIRS ? 4 : 8>(row + half + i, sn);
+    }
+    if (w && active) {
+      table_values<8>(w + d0, ww);
+      table_values<8>(w + partner, wp);
     }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int h = h0 + u * step;
-      if (h >= total) break;
-      const bool is_q = h < a.num_heads;
-      T* e16 = reinterpret_cast<T*>(&raw[u]);
-      float x[8], sum = 0.f;
+    for (int e = 0; e < 8; ++e) {
+      const float ce = !turn ? 1.f : PAIRS ? c[e >> 1] : c[e], se = !turn ? 0.f : PAIRS ? sn[e >> 1] : sn[e];
+      own[e] = ce * ww[e];
+      other[e] = ((PAIRS ? (e & 1) == 0 : d0 < half) ? -se : se) * (PAIRS ? wp[e ^ 1] : wp[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = d0 + e;
+      const bool turn = there && d < a.rot_dim;
+      const int i = !turn ? 0 : PAIRS ? d >> 1 : d < half ? d : d - half;
+      const int partner = !turn ? d : PAIRS ? d ^ 1 : d < half ? d + half : d - half;
+      const float c = turn ? table_value(row + i) : 1.f, sn = turn ? table_value(row + half + i) : 0.f;
+      own[e] = c * (w && active ? Ew<T>::to_f(w[d]) : 1.f);
+      other[e] = ((PAIRS ? (d & 1) == 0 : d < half) ? -sn : sn) * (w && active ? Ew<T>::to_f(w[partner]) : 1.f);
+    }
+  }
+  if (!there) return;
+#pragma unroll
+  for (int u = 0; u < kQkHeads; ++u) {
+    const int h = h0 + u * step;
+    if (h >= heads) break;
+    // The partners' inputs come over as they are, two to a word; their factor of the norm is this head's too.
+    uint4 them = raw[u];
+    if constexpr (MODE == kNeox) {
+      const int hl = half >> 3;
+      const int src = li < hl ? li + hl : li < 2 * hl ? li - hl : li;
+      them.x = __shfl_sync(lanes, raw[u].x, src, G);
+      them.y = __shfl_sync(lanes, raw[u].y, src, G);
+      them.z = __shfl_sync(lanes, raw[u].z, src, G);
+      them.w = __shfl_sync(lanes, raw[u].w, src, G);
+    } else if constexpr (MODE == kNeoxAny) {
+      swap[grp][li] = raw[u];
+      __syncwarp(lanes);
+      T* te = reinterpret_cast<T*>(&them);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = Ew<T>::to_f(e16[e]);
-        sum = fmaf(x[e], x[e], sum);
+        const int d = d0 + e;
+        te[e] = reinterpret_cast<const T*>(swap[grp])[d >= a.rot_dim ? d : d < half ? d + half : d - half];
       }
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
-      const float r = rsqrtf(sum / (float)a.head_size + a.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= r * (is_q ? wq[e] : wk[e]);
-      float y[8];
-      if (MODE == kPairs) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], c[e], x[e ^ 1] * s[e]);
-      } else if (MODE == kNeoxLanes) {
-        const int hl = half >> 3;
-        const int src = li < hl ? li + hl : li < 2 * hl ? li - hl : li;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], c[e], __shfl_sync(lanes, x[e], src, G) * s[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) swap[grp][d0 + e] = x[e];
-        __syncwarp(lanes);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = d0 + e;
-          const int from = d >= a.rot_dim ? d : d < half ? d + half : d - half;
-          y[e] = fmaf(x[e], c[e], swap[grp][from] * s[e]);
-        }
-        __syncwarp(lanes);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) e16[e] = Ew<T>::from_f(y[e]);
-      if (active) {
-        T* p = is_q ? static_cast<T*>(a.query_out) + t * a.qo_stride + (long long)h * a.head_size
-                    : static_cast<T*>(a.key_out) + t * a.ko_stride + (long long)(h - a.num_heads) * a.head_size;
-        *reinterpret_cast<uint4*>(p + d0) = raw[u];
-      }
+      __syncwarp(lanes);
     }
+    T* e16 = reinterpret_cast<T*>(&raw[u]);
+    const T* t16 = reinterpret_cast<const T*>(&them);
+    float x[8], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = Ew<T>::to_f(e16[e]);
+      sum = fmaf(x[e], x[e], sum);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
+    const float r = rsqrtf(sum / (float)a.head_size + a.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = PAIRS ? x[e ^ 1] : Ew<T>::to_f(t16[e]);
+      e16[e] = Ew<T>::from_f(fmaf(x[e], own[e], p * other[e]) * r);
+    }
+    if (active) *reinterpret_cast<uint4*>(out + (long long)h * a.head_size + d0) = raw[u];
   }
 }
 
 template <class T, class TC, int G>
 static void launch_qk_norm(const QkNormArgs& a, int mode, dim3 grid, cudaStream_t st) {
-  if (mode == kPairs) qk_norm_rotary_kernel<T, TC, G, kPairs><<<grid, kQkThreads, 0, st>>>(a);
-  else if (mode == kNeoxLanes) qk_norm_rotary_kernel<T, TC, G, kNeoxLanes><<<grid, kQkThreads, 0, st>>>(a);
-  else qk_norm_rotary_kernel<T, TC, G, kNeoxAny><<<grid, kQkThreads, 0, st>>>(a);
+  if (mode == kNeox) qk_norm_rotary_kernel<T, TC, G, kNeox><<<grid, kQkThreads, 0, st>>>(a);
+  else if (mode == kNeoxAny) qk_norm_rotary_kernel<T, TC, G, kNeoxAny><<<grid, kQkThreads, 0, st>>>(a);
+  else if (mode == kPairs) qk_norm_rotary_kernel<T, TC, G, kPairs><<<grid, kQkThreads, 0, st>>>(a);
+  else qk_norm_rotary_kernel<T, TC, G, kPairsAny><<<grid, kQkThreads, 0, st>>>(a);
 }
 
 template <class T, class TC>
 static void launch_qk_norm(const QkNormArgs& a, int num_tokens, bool is_neox, int sms, cudaStream_t st) {
   int g = 1;
   while (g * 8 < a.head_size) g *= 2;
-  const int groups = kQkThreads / g, total = a.num_heads + a.num_kv_heads;
-  // Few tokens: a token's heads go to several CTAs, down to one head per group, until about four CTAs per SM run.
-  const int most = (total + groups - 1) / groups;
-  int y = (4 * sms + num_tokens - 1) / num_tokens;
-  y = y < 1 ? 1 : y > most ? most : y;
-  const dim3 grid(num_tokens, y);
-  const int mode = !is_neox ? kPairs : a.rot_dim % 16 == 0 ? kNeoxLanes : kNeoxAny;
+  const int groups = kQkThreads / g, heads = a.num_heads > a.num_kv_heads ? a.num_heads : a.num_kv_heads;
+  // A CTA has the query's or the key's heads of a token, kQkHeads of them in a group; few tokens: fewer heads in a group,
+  // until about four CTAs per SM run.
+  const int most = (heads + groups - 1) / groups, least = (heads + kQkHeads * groups - 1) / (kQkHeads * groups);
+  int y = (2 * sms + num_tokens - 1) / num_tokens;
+  y = y < least ? least : y > most ? most : y;
+  const dim3 grid(num_tokens, y, a.num_kv_heads > 0 ? 2 : 1);
+  const bool aligned = (((uintptr_t)a.table | (uintptr_t)a.query_weight | (uintptr_t)a.key_weight) & 15) == 0;
+  const int mode = is_neox ? (aligned && a.rot_dim % 16 == 0 ? kNeox : kNeoxAny) : (aligned && a.rot_dim % 8 == 0 ? kPairs : kPairsAny);
   switch (g) {
     case 1: launch_qk_norm<T, TC, 1>(a, mode, grid, st); break;
     case 2: launch_qk_norm<T, TC, 2>(a, mode, grid, st); break;
