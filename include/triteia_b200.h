@@ -279,7 +279,11 @@ int trb_paged_attention(const void* query, const void* key_cache, const void* va
                         long long query_token_stride, long long query_head_stride, long long out_token_stride,
                         long long out_head_stride, long long page_stride, long long token_stride, long long head_stride,
                         long long exp_page_stride, long long exp_token_stride, long long exp_head_stride, float scale,
-                        int causal, int window, int dtype, int dev, void* stream);
+                        int causal, int window, int dtype, void* workspace, size_t workspace_bytes, int dev, void* stream);
+/* Working memory of that call (16-byte aligned, no initial contents needed, free again when the call has finished on the
+ * device): pieces of the sequences that more than one CTA reads.  single: query_starts is NULL; e4m3: there are exponents. */
+size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                           int page_size, int table_width, int single, int e4m3, int dev);
 
 /* sums[r] = (accumulate ? sums[r] : 0) + sum over n of y[r, n]: fp32 per-row checksum of an fp16
  * matrix [rows, prob_m] (prob_m % 8 == 0, y 16-byte aligned), fixed summation order.  Used by the

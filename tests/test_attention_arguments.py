@@ -28,7 +28,7 @@ def _attention(**change):
              out=64, num_tokens=3, num_seqs=2, num_heads=4, num_kv_heads=2, head_size=64, page_size=16, num_pages=4, table_stride=2,
              table_width=2, query_token_stride=256, query_head_stride=64, out_token_stride=256, out_head_stride=64, page_stride=2048,
              token_stride=128, head_stride=64, exp_page_stride=0, exp_token_stride=0, exp_head_stride=0, scale=0.125, causal=1, window=0,
-             dtype=0, dev=0, stream=None)
+             dtype=0, workspace=64, workspace_bytes=1 << 30, dev=0, stream=None)
     assert set(change) <= set(a)
     return _lib.lib.trb_paged_attention(*{**a, **change}.values())
 
@@ -39,7 +39,7 @@ def _attention(**change):
     (dict(num_seqs=-1), 3), (dict(num_heads=0), 3), (dict(num_kv_heads=0), 3), (dict(page_size=0), 3), (dict(num_pages=-1), 3),
     (dict(table_width=-1), 3), (dict(window=-1), 3), (dict(query_starts=None), 3),
     (dict(num_heads=5), 1), (dict(window=4, causal=0), 1), (dict(query=72), 1), (dict(out=72), 1), (dict(key_cache=72), 1),
-    (dict(value_cache=66), 1), (dict(query_token_stride=257), 1), (dict(out_head_stride=66), 1), (dict(token_stride=132), 1),
+    (dict(value_cache=66), 1), (dict(workspace=72), 1), (dict(query_token_stride=257), 1), (dict(out_head_stride=66), 1), (dict(token_stride=132), 1),
     (dict(table_width=1 << 28, page_size=64), 1), (dict(num_tokens=1 << 30, num_heads=8), 1),
     (dict(head_size=80), 2), (dict(head_size=256), 2), (dict(dtype=2), 2),
 ])

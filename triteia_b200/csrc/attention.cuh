@@ -14,8 +14,11 @@
 //   M = 16: the four warps of a CTA take different tokens (16 each of every 64) and keep softmax states of their own,
 //           so that nothing in the loop is CTA-wide; the states meet at the end.
 //   M = 64: a warp has 16 rows, and the four share the 64 tokens of a stage.
-// The CTAs of a cluster share a tile along the tokens and join their states through distributed shared memory: one
-// launch, no workspace, no counters, and a fixed order of the sums.
+// The work is cut evenly whatever the sequences' lengths: all (tile, key head) items' units of 64 or 128 tokens stand in one
+// line, every CTA of one resident wave takes an equal run of it, and the loads run ahead of the arithmetic across the items'
+// borders.  An item inside a run is finished there; of one that a border cuts, the pieces' states (maximum, sum, weighted
+// values) go to the caller's workspace, and a second launch joins them in the order of the tokens: no counters, nothing to
+// clear, a fixed order of the sums.
 // Loads are 16-byte cp.async with a row address per token (any page size and strides); a token outside the visible range
 // or on a page outside the cache is filled with zeros and masked.
 #pragma once
@@ -54,6 +57,12 @@ __device__ __forceinline__ void attn_query_range(const AttnArgs& a, int b, int& 
   }
   first = max(0, min(a.query_starts[b], a.tokens));
   last = max(first, min(a.query_starts[b + 1], a.tokens));
+}
+
+// Tokens in the cache, held within the page table.
+__device__ __forceinline__ int attn_length(const AttnArgs& a, int b) {
+  const long long most = (long long)a.table_width * a.page_size;
+  return (int)max(0LL, min((long long)a.lengths[b], most));
 }
 
 // The `index`-th tile of the batch; all lanes of a warp call it together.  False: there are fewer tiles.
@@ -98,8 +107,7 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs& a, int index, Att
   t.new_tokens = last - first;
   t.row0 = (index - before) * M;
   t.rows = min(M, t.new_tokens * a.group - t.row0);
-  const long long most = (long long)a.table_width * a.page_size;
-  t.length = (int)max(0LL, min((long long)a.lengths[t.seq], most));
+  t.length = attn_length(a, t.seq);
   return true;
 }
 
@@ -111,6 +119,122 @@ __device__ __forceinline__ void attn_key_range(const AttnArgs& a, const AttnTile
   if (a.causal) hi = min(hi, base + (t.row0 + t.rows - 1) / a.group + 1);
   if (a.window > 0) lo = max(0, base + t.row0 / a.group - a.window + 1);
   if (hi < lo) hi = lo;
+}
+
+// A tile and a key head: units [u0, u0 + n) of UNIT tokens, at least one (which may hold nothing that a row sees).
+struct AttnItem {
+  AttnTile t;
+  int kvh, lo, hi, u0, n;
+};
+
+template <int M, int UNIT>
+__device__ __forceinline__ void attn_item_units(const AttnArgs& a, AttnItem& it) {
+  attn_key_range(a, it.t, it.lo, it.hi);
+  it.u0 = it.lo / UNIT;
+  it.n = it.hi > it.lo ? (it.hi + UNIT - 1) / UNIT - it.u0 : 1;
+}
+
+// Units of one key head of sequence b.
+template <int M, int UNIT>
+__device__ __forceinline__ long long attn_seq_units(const AttnArgs& a, int b) {
+  AttnItem it;
+  if (a.query_starts == nullptr && a.group <= M) {    // one tile, and no divisions
+    const int hi = attn_length(a, b), lo = a.window > 0 ? max(0, hi - a.window) : 0;
+    return hi > lo ? (hi + UNIT - 1) / UNIT - lo / UNIT : 1;
+  }
+  int first, last;
+  attn_query_range(a, b, first, last);
+  it.t = AttnTile{b, 0, 0, first, last - first, attn_length(a, b)};
+  long long n = 0;
+  const int rows = (last - first) * a.group;
+  for (int r = 0; r < rows; r += M) {
+    it.t.row0 = r;
+    it.t.rows = min(M, rows - r);
+    attn_item_units<M, UNIT>(a, it);
+    n += it.n;
+  }
+  return n;
+}
+
+// The line's length in units; all lanes of a warp together.  `own`: the units of this lane's sequence among the first 32.
+template <int M, int UNIT>
+__device__ __forceinline__ long long attn_total_units(const AttnArgs& a, long long& own) {
+  const int lane = threadIdx.x & 31;
+  own = lane < a.seqs ? attn_seq_units<M, UNIT>(a, lane) : 0;
+  long long n = own;
+  for (int b = lane + 32; b < a.seqs; b += 32) n += attn_seq_units<M, UNIT>(a, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * a.kv_heads;
+}
+
+// First unit of CTA x's run of the line: total * x / ctas, with one wide division for all x (a wide one takes 100 clocks).
+struct AttnRuns {
+  long long each;
+  uint32_t left, ctas;
+  __device__ __forceinline__ AttnRuns(long long total, int n) : ctas((uint32_t)n) {
+    each = total <= 0xffffffffLL ? (long long)((uint32_t)total / ctas) : total / ctas;
+    left = (uint32_t)(total - each * ctas);
+  }
+  __device__ __forceinline__ long long begin(int x) const { return each * x + left * (uint32_t)x / ctas; }      // below ctas^2 < 2^32
+};
+
+// The item that holds unit `flat` of the line (flat < total) and the unit's number in it; all lanes of a warp together.
+template <int M, int UNIT>
+__device__ __forceinline__ int attn_seek(const AttnArgs& a, long long flat, long long own, AttnItem& it) {
+  const int lane = threadIdx.x & 31;
+  int b = 0;
+  for (int base = 0;; base += 32) {
+    const long long n = (base == 0 ? own : base + lane < a.seqs ? attn_seq_units<M, UNIT>(a, base + lane) : 0) * a.kv_heads;
+    long long inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, inc > flat);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      b = base + at;
+      flat -= __shfl_sync(0xffffffffu, inc - n, at);
+      break;
+    }
+    flat -= __shfl_sync(0xffffffffu, inc, 31);
+    if (base + 32 >= a.seqs) return 0;                // not reached: flat < total
+  }
+  int first, last;
+  attn_query_range(a, b, first, last);
+  it.t = AttnTile{b, 0, 0, first, last - first, attn_length(a, b)};
+  const int rows = (last - first) * a.group;
+  for (int r = 0; r < rows; r += M) {
+    it.t.row0 = r;
+    it.t.rows = min(M, rows - r);
+    attn_item_units<M, UNIT>(a, it);
+    const long long all = (long long)it.n * a.kv_heads;
+    if (flat < all) break;
+    flat -= all;
+  }
+  it.kvh = (int)(flat / it.n);
+  return (int)(flat - (long long)it.kvh * it.n);
+}
+
+// The next item of the line.  The caller knows that there is one.
+template <int M, int UNIT>
+__device__ __forceinline__ void attn_next(const AttnArgs& a, AttnItem& it) {
+  if (++it.kvh < a.kv_heads) return;
+  it.kvh = 0;
+  it.t.row0 += M;
+  if (it.t.row0 >= it.t.new_tokens * a.group) {
+    int first = 0, last = 0, b = it.t.seq;
+    do {
+      ++b;
+      if (b >= a.seqs) return;
+      attn_query_range(a, b, first, last);
+    } while (last <= first);
+    it.t = AttnTile{b, 0, 0, first, last - first, attn_length(a, b)};
+  }
+  it.t.rows = min(M, it.t.new_tokens * a.group - it.t.row0);
+  attn_item_units<M, UNIT>(a, it);
 }
 
 template <class T, bool FP8_, int D_, bool ROWS_>
@@ -129,10 +253,12 @@ struct AttnCfg {
   static constexpr int STAGES = 98304 / STAGE_BYTES > 6 ? 6 : 98304 / STAGE_BYTES;
   static constexpr int MASK_OFF = STAGES * STAGE_BYTES;         // uint32 [STAGES][4]: tokens that count, per loading warp
   static constexpr int EXP_OFF = MASK_OFF + STAGES * 16;        // float [STAGES][3][UNIT]: 2^e of keys; e and 2^-e of values
-  static constexpr int ML_OFF = EXP_OFF + (FP8 ? STAGES * 3 * UNIT * 4 : 0);   // float [M][2]: the CTA's maxima and sums
-  static constexpr int WML_OFF = ML_OFF + M * 8;                // float [4][16][2]: the warps' (M = 16)
-  static constexpr int SMEM_BYTES = WML_OFF + 4 * 16 * 8;
-  static constexpr int O_STRIDE = D + 4;                        // floats; rows of the joined states (in the idle ring)
+  static constexpr int WML_OFF = EXP_OFF + (FP8 ? STAGES * 3 * UNIT * 4 : 0);   // float [4][16][2]: the warps' maxima and sums (M = 16)
+  static constexpr int ML_OFF = WML_OFF + (ROWS ? 0 : 4 * 16 * 8);             // float [16][2]: the CTA's (M = 16)
+  static constexpr int O_STRIDE = D + 4;                                       // floats
+  static constexpr int O_OFF = ML_OFF + (ROWS ? 0 : 16 * 8);                   // float [16][O_STRIDE]: the CTA's weighted values
+  static constexpr int SMEM_BYTES = O_OFF + (ROWS ? 0 : 16 * O_STRIDE * 4);
+  static constexpr int PIECE_FLOATS = M * (D + 2);              // a piece in the workspace: values [M][D], maximum and sum [M][2]
   static constexpr int THREADS = 128;
 };
 
@@ -368,27 +494,61 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
   }
 }
 
-template <class T, class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a) {
+// A row's 4 or 8 numbers, divided by the sum and rounded once.
+template <class T, int N>
+__device__ __forceinline__ void attn_store_row(T* dst, const float* v, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int e = 0; e < N; e += 2) w[e / 2] = l == 0.f ? 0u : pack2(v[e] * inv, v[e + 1] * inv, T());
+  if constexpr (N == 2) *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T>
+__device__ __forceinline__ T* attn_out_row(const AttnArgs& a, const AttnItem& it, int row) {
+  const int rq = it.t.row0 + row, i = rq / a.group, head = it.kvh * a.group + (rq - i * a.group);
+  return static_cast<T*>(a.out) + (long long)(it.t.q0 + i) * a.o_tok + (long long)head * a.o_head;
+}
+
+// CLUSTER: a cluster shares one item (of a single-token call) instead, its CTAs' states meet through distributed shared memory,
+// and there is no line to cut and no second launch.
+template <class T, class Cfg, bool CLUSTER>
+__global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a, float* pieces) {
   using TM = typename AttnMma<T, Cfg::FP8>::type;
-  constexpr int D = Cfg::D, M = Cfg::M, STAGES = Cfg::STAGES;
+  constexpr int D = Cfg::D, M = Cfg::M, STAGES = Cfg::STAGES, UNIT = Cfg::UNIT;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t smem_base = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3;
-  uint32_t parts, part;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
-  const int item = blockIdx.x / parts;
-  const int kvh = item % a.kv_heads;
-  AttnTile t;
-  if (!attn_find_tile<M>(a, item / a.kv_heads, t)) return;      // the whole cluster leaves
-  int lo, hi;
-  attn_key_range(a, t, lo, hi);
-  // This CTA's units of 64 tokens.
-  const int u_first = lo / Cfg::UNIT, u_all = hi > lo ? (hi + Cfg::UNIT - 1) / Cfg::UNIT - u_first : 0;
-  const int u0 = u_first + (int)((long long)u_all * part / parts), u1 = u_first + (int)((long long)u_all * (part + 1) / parts);
+  AttnItem it;                          // the item that is computed
+  int skip;
+  long long f0, f1;                     // this CTA's run of the line (CLUSTER: of the item)
+  uint32_t parts = 1, part = 0;
+  if constexpr (CLUSTER) {
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+    const int item = blockIdx.x / parts;
+    attn_find_tile<M>(a, item / a.kv_heads, it.t);
+    it.kvh = item % a.kv_heads;
+    attn_item_units<M, UNIT>(a, it);
+    skip = (int)((uint32_t)it.n * part / parts);
+    f0 = skip;
+    f1 = (uint32_t)it.n * (part + 1) / parts;
+  } else {
+    pdl_launch_dependents();            // the joining launch waits for this one's end before it reads
+    long long own;
+    const long long total = attn_total_units<M, UNIT>(a, own);
+    const AttnRuns runs(total, gridDim.x);
+    f0 = runs.begin(blockIdx.x);
+    f1 = runs.begin(blockIdx.x + 1);
+    if (f0 == f1) return;
+    skip = attn_seek<M, UNIT>(a, f0, own, it);
+  }
+  long long flat = f0 - skip;           // the item's place in the line
+  AttnItem ld = it;                     // the item whose loads are issued
+  int ld_u = it.u0 + skip;
+  long long ld_left = f1 - f0;          // units whose loads have not been issued
 
-  const int* table = a.page_table + t.seq * a.table_stride;
   const uint8_t* kc = static_cast<const uint8_t*>(a.key_cache);
   const uint8_t* vc = static_cast<const uint8_t*>(a.value_cache);
   constexpr int ESZ = Cfg::FP8 ? 1 : 2;
@@ -397,37 +557,42 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
   constexpr int WTOK = Cfg::WTOK;                     // 16 or 32 tokens of a stage are this warp's to load
   const int tok = warp * WTOK + (lane & (WTOK - 1));  // this lane's among the unit's
 
-  // Page and place of this lane's token of unit u (page -1: not visible, or not in the cache), found one unit ahead.
-  struct Where { int page, place; };
-  auto where = [&](int u) -> Where {
-    const int j = u * Cfg::UNIT + tok;
-    if (u >= u1 || j < lo || j >= hi) return {-1, 0};
+  // Page, place and key head of this lane's token of unit ld_u (page -1: not visible, or not in the cache), found one unit ahead.
+  struct Where { int page, place, kvh; };
+  auto where = [&]() -> Where {
+    const int j = ld_u * UNIT + tok;
+    if (ld_left == 0 || j < ld.lo || j >= ld.hi) return {-1, 0, 0};
     const int p = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-    const int pg = table[p];
-    return {pg >= 0 && pg < a.num_pages ? pg : -1, j - p * a.page_size};
+    const int pg = a.page_table[ld.t.seq * a.table_stride + p];
+    return {pg >= 0 && pg < a.num_pages ? pg : -1, j - p * a.page_size, ld.kvh};
   };
-  Where ahead = where(u0);
+  Where ahead = where();
   int exp_slot = -1, kb = 127, vb = 127;              // e4m3: the bytes that the last issue() asked for, and their stage
   auto settle_exps = [&]() {
     if (exp_slot >= 0 && lane < WTOK) {
-      float* e = exps + exp_slot * 3 * Cfg::UNIT + tok;
+      float* e = exps + exp_slot * 3 * UNIT + tok;
       e[0] = pow2_of_byte(kb);
-      e[Cfg::UNIT] = (float)(vb - 127);
-      e[2 * Cfg::UNIT] = pow2_of_byte(254 - vb);
+      e[UNIT] = (float)(vb - 127);
+      e[2 * UNIT] = pow2_of_byte(254 - vb);
     }
   };
   constexpr int PER = 32 / Cfg::CHUNKS;               // rows per instruction
   const int c = lane % Cfg::CHUNKS, r0 = lane / Cfg::CHUNKS;
   const long long row_bytes = a.c_tok * ESZ;
   const bool paged16 = (a.page_size & 15) == 0;       // 16 tokens of a unit lie on one page
-  // Loads this warp's tokens of unit u into `slot`.
-  auto issue = [&](int u, int slot) {
+  // Loads this warp's tokens of the next unit into `slot`.
+  auto issue = [&](int slot) {
     if constexpr (Cfg::FP8) settle_exps();
-    const Where w = ahead;
-    ahead = where(u + 1);
-    if (u < u1) {
+    exp_slot = -1;
+    if (ld_left > 0) {
+      const Where w = ahead;
+      if (--ld_left > 0 && ++ld_u == ld.u0 + ld.n) {
+        attn_next<M, UNIT>(a, ld);
+        ld_u = ld.u0;
+      }
+      ahead = where();
       const bool there = w.page >= 0;
-      long long off = there ? (long long)w.page * a.c_page + (long long)w.place * a.c_tok + (long long)kvh * a.c_head : 0;
+      long long off = there ? (long long)w.page * a.c_page + (long long)w.place * a.c_tok + (long long)w.kvh * a.c_head : 0;
       if constexpr (ESZ == 2) off *= 2;
       unsigned mask = __ballot_sync(0xffffffffu, there);
       if constexpr (WTOK == 16) mask &= 0xffffu;
@@ -436,7 +601,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
         exp_slot = slot;
         kb = vb = 127;
         if (there) {
-          const long long eo = (long long)w.page * a.e_page + (long long)w.place * a.e_tok + (long long)kvh * a.e_head;
+          const long long eo = (long long)w.page * a.e_page + (long long)w.place * a.e_tok + (long long)w.kvh * a.e_head;
           kb = a.key_exp[eo];
           vb = a.value_exp[eo];
         }
@@ -467,231 +632,334 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a)
           cp_async16(at + Cfg::HALF_BYTES, vc + ro, ok);
         }
       }
-    } else {
-      exp_slot = -1;
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(u0 + i, i);
-
-  // ---- this warp's rows: query fragments, visible ranges
-  const int wrow = Cfg::ROWS ? warp * 16 : 0;
-  uint32_t q[D / 16][4];
-  float c_row[2];
-  int row_hi[2], row_lo[2];
-#pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const int row = wrow + (lane >> 2) + 8 * rr;
-    const bool on = row < t.rows;
-    const int rq = t.row0 + (on ? row : 0);
-    const int i = rq / a.group, head = kvh * a.group + (rq - i * a.group);
-    const T* qp = static_cast<const T*>(a.query) + (t.q0 + i) * a.q_tok + head * a.q_head;
-    const int pos = t.length - t.new_tokens + i;
-    row_hi[rr] = a.causal ? min(hi, pos + 1) : hi;
-    row_lo[rr] = a.window > 0 ? pos - a.window + 1 : 0;
-    c_row[rr] = a.scale_log2;
-    if constexpr (!Cfg::FP8) {
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          q[ks][rr + 2 * h] = on ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + 2 * quad) : 0u;
-    } else {
-      float top = 0.f;
-      uint2 raw[D / 16];
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        raw[ks] = on ? *reinterpret_cast<const uint2*>(qp + ks * 16 + 4 * quad) : make_uint2(0, 0);
-        const T* e = reinterpret_cast<const T*>(&raw[ks]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) top = fmaxf(top, fabsf(Ew<T>::to_f(e[x])));
-      }
-      float up = 1.f;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int k = attn_row_shift(top);
-        up = __uint_as_float((uint32_t)k << 23);
-        c_row[rr] *= __uint_as_float((uint32_t)(254 - k) << 23);
-      }
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const T* e = reinterpret_cast<const T*>(&raw[ks]);
-        q[ks][rr] = pack2(Ew<T>::to_f(e[0]) * up, Ew<T>::to_f(e[1]) * up, __half());
-        q[ks][rr + 2] = pack2(Ew<T>::to_f(e[2]) * up, Ew<T>::to_f(e[3]) * up, __half());
-      }
-    }
-  }
-  AttnState<D> st;
-#pragma unroll
-  for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) st.o[d][e] = 0.f;
-  st.m[0] = st.m[1] = -INFINITY;
-  st.l[0] = st.l[1] = 0.f;
-  // Tokens [all_lo, all_hi) are seen by every row of the warp.
-  const int base_pos = t.length - t.new_tokens;
-  const int last_row = min(wrow + 15, t.rows - 1);
-  const int all_hi = a.causal ? min(hi, base_pos + (t.row0 + wrow) / a.group + 1) : hi;
-  const int all_lo = a.window > 0 ? base_pos + (t.row0 + last_row) / a.group - a.window + 1 : 0;
-  const bool idle = wrow >= t.rows;
+  for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
   int slot = 0;
-  for (int u = u0; u < u1; ++u) {
-    cp_async_wait<STAGES - 2>();
-    if constexpr (Cfg::ROWS) __syncthreads();
-    else __syncwarp();
-    issue(u + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-    if (!idle) {
-      constexpr int TOK = Cfg::NT * 16;
-      const int own = Cfg::ROWS ? 0 : warp * WTOK;
-      const int j0 = u * Cfg::UNIT + own;
-      const uint32_t* mk = masks + slot * 4;
-      const unsigned long long valid =
-          Cfg::ROWS ? (unsigned long long)(mk[0] | mk[1] << 16) | (unsigned long long)(mk[2] | mk[3] << 16) << 32 : mk[warp];
-      constexpr unsigned long long kAll = ~0ull >> (64 - TOK);
-      if (valid != 0) {
-        const bool need_mask = valid != kAll || j0 + TOK > all_hi || j0 < all_lo;
-        const uint32_t kbase = smem_base + slot * Cfg::STAGE_BYTES + own * Cfg::ROWB;
-        attn_block<T, Cfg, Cfg::NT>(st, q, c_row, kbase, kbase + Cfg::HALF_BYTES, exps + slot * 3 * Cfg::UNIT + own, valid, j0, row_hi,
-                                    row_lo, need_mask, lane);
-      }
-    }
-    if constexpr (!Cfg::ROWS) __syncwarp();
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
-  }
-  cp_async_wait<0>();
-  __syncthreads();                      // the ring is idle: it takes the states now
-
-  // ---- states into shared memory: float o[rows][D + 4], {m, l} per row
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
-  }
-  float* obuf = reinterpret_cast<float*>(smem);
-  float2* ml = reinterpret_cast<float2*>(smem + Cfg::ML_OFF);
-  float2* wml = reinterpret_cast<float2*>(smem + Cfg::WML_OFF);
-  {
+  for (long long f = f0; f < f1 || CLUSTER;) {        // CLUSTER: one round, with nothing in it if the share is empty
+    // ---- a piece: units [u, u_end) of item `it`
+    int u = it.u0 + (int)(f - flat);
+    const int u_end = (int)min((long long)(it.u0 + it.n), u + (f1 - f));
+    const bool whole = u == it.u0 && u_end == it.u0 + it.n;
+    const AttnTile& t = it.t;
+    const int hi = it.hi;
+    // this warp's rows: query fragments, visible ranges
+    const int wrow = Cfg::ROWS ? warp * 16 : 0;
+    uint32_t q[D / 16][4];
+    float c_row[2];
+    int row_hi[2], row_lo[2];
 #pragma unroll
     for (int rr = 0; rr < 2; ++rr) {
-      const int row = warp * 16 + (lane >> 2) + 8 * rr;
-      float* dst = obuf + row * Cfg::O_STRIDE;
-      if (quad == 0) (Cfg::ROWS ? ml : wml)[row] = make_float2(st.m[rr], st.l[rr]);
+      const int row = wrow + (lane >> 2) + 8 * rr;
+      const bool on = row < t.rows;
+      const int rq = t.row0 + (on ? row : 0);
+      const int i = rq / a.group, head = it.kvh * a.group + (rq - i * a.group);
+      const T* qp = static_cast<const T*>(a.query) + (long long)(t.q0 + i) * a.q_tok + (long long)head * a.q_head;
+      const int pos = t.length - t.new_tokens + i;
+      row_hi[rr] = a.causal ? min(hi, pos + 1) : hi;
+      row_lo[rr] = a.window > 0 ? pos - a.window + 1 : 0;
+      c_row[rr] = a.scale_log2;
       if constexpr (!Cfg::FP8) {
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-          *reinterpret_cast<float2*>(dst + d * 8 + 2 * quad) = make_float2(st.o[d][2 * rr], st.o[d][2 * rr + 1]);
-      } else {
+        for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-          *reinterpret_cast<float4*>(dst + d * 16 + 4 * quad) =
-              make_float4(st.o[2 * d][2 * rr], st.o[2 * d + 1][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr + 1]);
+          for (int h = 0; h < 2; ++h)
+            q[ks][rr + 2 * h] = on ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + 2 * quad) : 0u;
+      } else {
+        float top = 0.f;
+        uint2 raw[D / 16];
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          raw[ks] = on ? *reinterpret_cast<const uint2*>(qp + ks * 16 + 4 * quad) : make_uint2(0, 0);
+          const T* e = reinterpret_cast<const T*>(&raw[ks]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) top = fmaxf(top, fabsf(Ew<T>::to_f(e[x])));
+        }
+        float up = 1.f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int k = attn_row_shift(top);
+          up = __uint_as_float((uint32_t)k << 23);
+          c_row[rr] *= __uint_as_float((uint32_t)(254 - k) << 23);
+        }
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const T* e = reinterpret_cast<const T*>(&raw[ks]);
+          q[ks][rr] = pack2(Ew<T>::to_f(e[0]) * up, Ew<T>::to_f(e[1]) * up, __half());
+          q[ks][rr + 2] = pack2(Ew<T>::to_f(e[2]) * up, Ew<T>::to_f(e[3]) * up, __half());
+        }
       }
     }
-  }
-  __syncthreads();
-  if constexpr (!Cfg::ROWS) {
-    // The four warps' states become the CTA's, in place of the first warp's: an element is read and written by one thread.
-    for (int x = tid; x < 16 * (D / 4); x += Cfg::THREADS) {
-      const int row = x / (D / 4), d = (x % (D / 4)) * 4;
-      float m = -INFINITY;
+    AttnState<D> st;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) m = fmaxf(m, wml[w * 16 + row].x);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[d][e] = 0.f;
+    st.m[0] = st.m[1] = -INFINITY;
+    st.l[0] = st.l[1] = 0.f;
+    // Tokens [all_lo, all_hi) are seen by every row of the warp.
+    const int base_pos = t.length - t.new_tokens;
+    const int last_row = min(wrow + 15, t.rows - 1);
+    const int all_hi = a.causal ? min(hi, base_pos + (t.row0 + wrow) / a.group + 1) : hi;
+    const int all_lo = a.window > 0 ? base_pos + (t.row0 + last_row) / a.group - a.window + 1 : 0;
+    const bool idle = wrow >= t.rows;
+
+    f += u_end - u;
+    for (; u < u_end; ++u) {
+      cp_async_wait<STAGES - 2>();
+      if constexpr (Cfg::ROWS) __syncthreads();
+      else __syncwarp();
+      issue(slot == 0 ? STAGES - 1 : slot - 1);
+      if (!idle) {
+        constexpr int TOK = Cfg::NT * 16;
+        const int own = Cfg::ROWS ? 0 : warp * WTOK;
+        const int j0 = u * UNIT + own;
+        const uint32_t* mk = masks + slot * 4;
+        const unsigned long long valid =
+            Cfg::ROWS ? (unsigned long long)(mk[0] | mk[1] << 16) | (unsigned long long)(mk[2] | mk[3] << 16) << 32 : mk[warp];
+        constexpr unsigned long long kAll = ~0ull >> (64 - TOK);
+        if (valid != 0) {
+          const bool need_mask = valid != kAll || j0 + TOK > all_hi || j0 < all_lo;
+          const uint32_t kbase = smem_base + slot * Cfg::STAGE_BYTES + own * Cfg::ROWB;
+          attn_block<T, Cfg, Cfg::NT>(st, q, c_row, kbase, kbase + Cfg::HALF_BYTES, exps + slot * 3 * UNIT + own, valid, j0, row_hi, row_lo,
+                                      need_mask, lane);
+        }
+      }
+      if constexpr (!Cfg::ROWS) __syncwarp();
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+
+    // ---- the piece's state: to the output, or to the workspace (slot 2 c of CTA c for the item its run begins in, or with;
+    // 2 c + 1 for another one)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
+      st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
+    }
+    float* piece = pieces + (2LL * blockIdx.x + (f0 < flat ? 1 : 0)) * Cfg::PIECE_FLOATS;
+    if constexpr (Cfg::ROWS) {
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        const int row = wrow + (lane >> 2) + 8 * rr;
+        if (row >= t.rows) continue;
+        T* dst = attn_out_row<T>(a, it, row);
+        if (!whole && quad == 0) *reinterpret_cast<float2*>(piece + M * D + 2 * row) = make_float2(st.m[rr], st.l[rr]);
+        constexpr int N = Cfg::FP8 ? 4 : 2;           // neighbouring sizes that a lane has
+#pragma unroll
+        for (int d = 0; d < D / (4 * N); ++d) {
+          float v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = Cfg::FP8 ? st.o[2 * d + (e & 1)][2 * rr + (e >> 1)] : st.o[d][2 * rr + e];
+          const int at = d * 4 * N + N * quad;
+          if (whole) attn_store_row<T, N>(dst + at, v, st.l[rr]);
+          else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) piece[row * D + at + e] = v[e];
+          }
+        }
+      }
+    } else {
+      float* obuf = reinterpret_cast<float*>(smem + Cfg::O_OFF);
+      float2* ml = reinterpret_cast<float2*>(smem + Cfg::ML_OFF);
+      float2* wml = reinterpret_cast<float2*>(smem + Cfg::WML_OFF);
+      if (quad == 0) {
+        wml[warp * 16 + (lane >> 2)] = make_float2(st.m[0], st.l[0]);
+        wml[warp * 16 + (lane >> 2) + 8] = make_float2(st.m[1], st.l[1]);
+      }
+      __syncthreads();
+      float f_row[2];
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        const int row = (lane >> 2) + 8 * rr;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, wml[w * 16 + row].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 s = wml[w * 16 + row];
+          if (s.x != -INFINITY) l = fmaf(s.y, exp2_fast(s.x - m), l);
+        }
+        f_row[rr] = st.m[rr] == -INFINITY ? 0.f : exp2_fast(st.m[rr] - m);
+        if (warp == 0 && quad == 0) ml[row] = make_float2(m, l);
+      }
+      // The warps add their parts one after the other: a fixed order.
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float2 s = wml[w * 16 + row];
-        const float f = s.x == -INFINITY ? 0.f : exp2_fast(s.x - m);
-        const float4 v = *reinterpret_cast<const float4*>(obuf + (w * 16 + row) * Cfg::O_STRIDE + d);
-        l = fmaf(s.y, f, l);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
-      }
-      *reinterpret_cast<float4*>(obuf + row * Cfg::O_STRIDE + d) = o;
-      if (d == 0) ml[row] = make_float2(m, l);
-    }
-  }
-  if (parts > 1) cluster_sync_all();
-  else __syncthreads();
-  // ---- the cluster's states joined in the order of the tokens, divided, rounded once
-  const uint32_t o_local = smem_base, ml_local = smem_base + Cfg::ML_OFF;
-  for (int x = (int)part * Cfg::THREADS + tid; x < t.rows * (D / 8); x += (int)parts * Cfg::THREADS) {
-    const int row = x / (D / 8), d = (x % (D / 8)) * 8;
-    float m = -INFINITY;
-    for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, ld_cluster_f32(mapa_shared(ml_local + row * 8, p)));
-    float o[8] = {}, l = 0.f;
-    if (m != -INFINITY) {
-      for (uint32_t p = 0; p < parts; ++p) {
-        const float f = exp2_fast(ld_cluster_f32(mapa_shared(ml_local + row * 8, p)) - m);
-        l = fmaf(ld_cluster_f32(mapa_shared(ml_local + row * 8 + 4, p)), f, l);
-        const uint32_t src = mapa_shared(o_local + (row * Cfg::O_STRIDE + d) * 4, p);
-        const float4 v0 = ld_cluster_f32x4(src), v1 = ld_cluster_f32x4(src + 16);
-        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+        if (warp == w) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
+          for (int rr = 0; rr < 2; ++rr) {
+            float* dst = obuf + ((lane >> 2) + 8 * rr) * Cfg::O_STRIDE;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              // Sizes 4 quad .. + 3 of each 16 (e4m3), or 2 quad, + 1 of each 8.
+              float4 v = Cfg::FP8 ? make_float4(st.o[2 * d][2 * rr], st.o[2 * d + 1][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr + 1])
+                                  : make_float4(st.o[2 * d][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr], st.o[2 * d + 1][2 * rr + 1]);
+              v = make_float4(v.x * f_row[rr], v.y * f_row[rr], v.z * f_row[rr], v.w * f_row[rr]);
+              float2* p0 = reinterpret_cast<float2*>(dst + d * 16 + (Cfg::FP8 ? 4 : 2) * quad);
+              float2* p1 = Cfg::FP8 ? p0 + 1 : p0 + 4;
+              if (w > 0) {
+                v.x += p0->x, v.y += p0->y;
+                v.z += p1->x, v.w += p1->y;
+              }
+              *p0 = make_float2(v.x, v.y);
+              *p1 = make_float2(v.z, v.w);
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if constexpr (CLUSTER) {
+        cluster_sync_all();
+        const uint32_t o_at = smem_base + Cfg::O_OFF, ml_at = smem_base + Cfg::ML_OFF;
+        for (int x = (int)part * Cfg::THREADS + tid; x < t.rows * (D / 8); x += (int)parts * Cfg::THREADS) {
+          const int row = x / (D / 8), d = (x % (D / 8)) * 8;
+          float m = -INFINITY, v[8] = {}, l = 0.f;
+          for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, ld_cluster_f32(mapa_shared(ml_at + row * 8, p)));
+          if (m != -INFINITY) {
+            for (uint32_t p = 0; p < parts; ++p) {
+              const float f_p = exp2_fast(ld_cluster_f32(mapa_shared(ml_at + row * 8, p)) - m);
+              l = fmaf(ld_cluster_f32(mapa_shared(ml_at + row * 8 + 4, p)), f_p, l);
+              const uint32_t src = mapa_shared(o_at + (row * Cfg::O_STRIDE + d) * 4, p);
+              const float4 w0 = ld_cluster_f32x4(src), w1 = ld_cluster_f32x4(src + 16);
+              const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = fmaf(w[e], f_p, v[e]);
+            }
+          }
+          attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
+        }
+        cluster_sync_all();             // nobody's shared memory goes before its neighbours have read it
+        break;
+      }
+      for (int x = tid; x < t.rows * (D / 8); x += Cfg::THREADS) {
+        const int row = x / (D / 8), d = (x % (D / 8)) * 8;
+        const float4 v0 = *reinterpret_cast<const float4*>(obuf + row * Cfg::O_STRIDE + d),
+                     v1 = *reinterpret_cast<const float4*>(obuf + row * Cfg::O_STRIDE + d + 4);
+        if (whole) {
+          const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+          attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, ml[row].y);
+        } else {
+          *reinterpret_cast<float4*>(piece + row * D + d) = v0;
+          *reinterpret_cast<float4*>(piece + row * D + d + 4) = v1;
+          if (d == 0) *reinterpret_cast<float2*>(piece + M * D + 2 * row) = ml[row];
+        }
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint4 packed;
-    T* pe = reinterpret_cast<T*>(&packed);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) pe[e] = Ew<T>::from_f(l == 0.f ? 0.f : o[e] * inv);
-    const int rq = t.row0 + row, i = rq / a.group, head = kvh * a.group + (rq - i * a.group);
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (t.q0 + i) * a.o_tok + head * a.o_head + d) = packed;
+    flat += it.n;
+    if (f < f1) attn_next<M, UNIT>(a, it);
   }
-  if (parts > 1) cluster_sync_all();    // nobody's shared memory goes before its neighbours have read it
+  cp_async_wait<0>();
 }
 
-// CTAs of a cluster that share a tile: where the tiles alone would leave SMs idle (two CTAs fit an SM), as many as fill
-// one wave, at most 16; several waves of tiles are cut into eight or so, so that sequences of different lengths even out.
-static int attn_parts(long long tiles, long long most_tokens, int unit, int sms) {
-  const long long slots = 2LL * sms, units = (most_tokens + unit - 1) / unit;
-  long long parts = 2 * tiles <= slots ? slots / tiles : (8 * slots + tiles - 1) / tiles;
-  parts = parts > 16 ? 16 : parts;
-  if (2 * tiles > slots && parts > 8) parts = 8;
-  if (parts > (units + 1) / 2) parts = (units + 1) / 2;      // two units each at least
-  return parts < 1 ? 1 : (int)parts;
+// Joins the pieces of the items that a border of two CTAs' runs cuts; `ctas`: the grid of the launch before.  CTA (c, y) has
+// part y of the item that the end of run c cuts first.
+template <class T, class Cfg>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const float* pieces, int ctas) {
+  constexpr int D = Cfg::D, M = Cfg::M, UNIT = Cfg::UNIT;
+  long long own;
+  const long long total = attn_total_units<M, UNIT>(a, own);
+  const int c = blockIdx.x;
+  const AttnRuns runs(total, ctas);
+  const long long border = runs.begin(c + 1);
+  AttnItem it = {};
+  int at = 0;
+  if (border < total && runs.begin(c) < border) at = attn_seek<M, UNIT>(a, border, own, it);
+  pdl_wait();                                         // the pieces are there; and this launch never ends before that one
+  const long long s = border - at, e = s + it.n;
+  if (at == 0 || runs.begin(c) > s) return;                // nothing is cut here, or an earlier border cuts it too
+  const int x = blockIdx.y * 128 + threadIdx.x;
+  if (x >= it.t.rows * (D / 8)) return;
+  const int row = x / (D / 8), d = (x % (D / 8)) * 8;
+  // Pieces of CTAs c .. c + n - 1; an empty run (fewer units than CTAs) has none.
+  int n = 1;
+  while (runs.begin(c + n) < e) ++n;
+  const float* first = pieces + (2LL * c + (runs.begin(c) < s ? 1 : 0)) * Cfg::PIECE_FLOATS;
+  const float* rest = pieces + 2LL * c * Cfg::PIECE_FLOATS;
+  auto piece_of = [&](int k) { return k == 0 ? first : rest + 2LL * k * Cfg::PIECE_FLOATS; };
+  auto held = [&](int k) { return runs.each > 0 || runs.begin(c + k + 1) > runs.begin(c + k); };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int k = 0; k < n; ++k)
+    if (held(k)) m = fmaxf(m, piece_of(k)[M * D + 2 * row]);
+  float v[8] = {}, l = 0.f;
+  if (m != -INFINITY) {
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      if (!held(k)) continue;
+      const float* p = piece_of(k);
+      const float2 ml = *reinterpret_cast<const float2*>(p + M * D + 2 * row);
+      const float4 v0 = *reinterpret_cast<const float4*>(p + row * D + d), v1 = *reinterpret_cast<const float4*>(p + row * D + d + 4);
+      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+      l = fmaf(ml.y, f, l);
+      const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = fmaf(w[i], f, v[i]);
+    }
+  }
+  attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
+}
+
+// How a call is cut.  ctas > 0: runs of the line, one wave of two CTAs per SM.  parts > 0: clusters of that many.
+struct AttnCut {
+  int ctas, parts;
+  long long items;
+};
+template <class Cfg>
+static AttnCut attn_cut(long long tokens, int seqs, int group, int kv_heads, bool single, long long most_tokens, int sms) {
+  const long long rows = tokens * group, per_token = (group + Cfg::M - 1) / Cfg::M;
+  // Tiles of the batch: at most one per token (or several where a group has more than M heads), and at most the full
+  // ones and one more per sequence.
+  long long tiles = single ? seqs * per_token : rows / Cfg::M + seqs;
+  if (!single && tiles > tokens * per_token) tiles = tokens * per_token;
+  const long long items = tiles * kv_heads, each = most_tokens > 0 ? (most_tokens + Cfg::UNIT - 1) / Cfg::UNIT : 1, slots = 2LL * sms;
+  // Short single-token calls: a cluster of up to eight CTAs for each item, all of them resident at once, at least two units
+  // and at most kShort for each CTA by the page table's width.
+  constexpr int kShort = 8;
+  if (single && !Cfg::ROWS && items * 2 <= slots) {
+    long long parts = slots / items < 8 ? slots / items : 8;
+    if (parts > (each + 1) / 2) parts = (each + 1) / 2;
+    if (parts >= 1 && each <= kShort * parts) return {0, (int)parts, items};
+  }
+  const long long ctas = items * each / 2 < slots ? items * each / 2 : slots;
+  return {ctas < 1 ? 1 : (int)ctas, 0, items};
 }
 
 template <class T, class Cfg>
-static int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
-  static std::atomic<bool> wide[64], done[64];
-  if (dev < 0 || dev >= 64 || !wide[dev].load(std::memory_order_acquire)) {      // clusters of more than eight CTAs
-    if (cudaFuncSetAttribute(attn_kernel<T, Cfg>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return TRB_ERR_CUDA;
-    if (dev >= 0 && dev < 64) wide[dev].store(true, std::memory_order_release);
-  }
-  if (!ensure_smem_attr(attn_kernel<T, Cfg>, dev, Cfg::SMEM_BYTES, done)) return TRB_ERR_CUDA;
-  const long long rows = (long long)a.tokens * a.group;
-  const long long per_token = (a.group + Cfg::M - 1) / Cfg::M;
-  // Tiles of the batch: at most one per token (or several where a group has more than M heads), and at most the full
-  // ones and one more per sequence.
-  long long tiles = a.query_starts ? rows / Cfg::M + a.seqs : a.seqs * per_token;
-  if (a.query_starts && tiles > a.tokens * per_token) tiles = a.tokens * per_token;
-  if (tiles == 0) return TRB_OK;
-  const int parts = attn_parts(tiles * a.kv_heads, (long long)a.table_width * a.page_size, Cfg::UNIT, sm_count(dev));
-  const long long grid = tiles * a.kv_heads * parts;
-  if (grid > 0x7fffffffLL) return TRB_ERR_PROB_SHAPE;
+static int launch_attn(const AttnArgs& a, void* workspace, size_t workspace_bytes, int dev, cudaStream_t st) {
+  const AttnCut cut = attn_cut<Cfg>(a.tokens, a.seqs, a.group, a.kv_heads, a.query_starts == nullptr, (long long)a.table_width * a.page_size,
+                                    sm_count(dev));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(Cfg::THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = st;
   cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = parts;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, attn_kernel<T, Cfg>, a) != cudaSuccess) {
-    cudaGetLastError();
-    return TRB_ERR_CUDA;
+  if constexpr (!Cfg::ROWS) {
+    if (cut.parts > 0) {
+      static std::atomic<bool> done[64];
+      if (!ensure_smem_attr(attn_kernel<T, Cfg, true>, dev, Cfg::SMEM_BYTES, done)) return TRB_ERR_CUDA;
+      cfg.gridDim = dim3((unsigned)(cut.items * cut.parts));
+      cfg.blockDim = dim3(Cfg::THREADS);
+      cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = cut.parts;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      return cudaLaunchKernelEx(&cfg, attn_kernel<T, Cfg, true>, a, (float*)nullptr) == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
+    }
   }
-  return TRB_OK;
+  static std::atomic<bool> done[64];
+  if (!ensure_smem_attr(attn_kernel<T, Cfg, false>, dev, Cfg::SMEM_BYTES, done)) return TRB_ERR_CUDA;
+  if (cut.ctas > 1 && (workspace == nullptr || workspace_bytes < 2ull * cut.ctas * Cfg::PIECE_FLOATS * 4)) return TRB_ERR_SCRATCH;
+  attn_kernel<T, Cfg, false><<<cut.ctas, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a, (float*)workspace);
+  if (cudaGetLastError() != cudaSuccess) return TRB_ERR_CUDA;
+  if (cut.ctas == 1) return TRB_OK;
+  cfg.gridDim = dim3(cut.ctas - 1, Cfg::M * (Cfg::D / 8) / 128);
+  cfg.blockDim = dim3(128);
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<T, Cfg>, a, (const float*)workspace, cut.ctas) == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
 }
-
 }  // namespace trb

@@ -5,29 +5,54 @@
 
 namespace trb {
 
+// Which kernel takes a call.  From 128 rows (token, query head of a group) of an average sequence on the matrix products
+// bound it; up to 16 rows the warps of a CTA split the tokens, beyond that the rows.
+enum AttnKind { kAttnSplit, kAttnRows, kAttnTensor };
+static AttnKind attn_kind(long long tokens, int seqs, int group, bool single, bool tensor_fits) {
+  const long long rows = single ? (long long)group * seqs : tokens * group;
+  if (!single && rows >= 128LL * seqs && tensor_fits) return kAttnTensor;
+  return rows > 16LL * seqs ? kAttnRows : kAttnSplit;
+}
+
+// Calls f with the configuration of the kernel for short calls.
+template <class T, class F>
+static auto attn_with_cfg(bool fp8, int head_size, bool rows, F f) {
+  if (head_size == 128) {
+    if (fp8) return rows ? f(AttnCfg<T, true, 128, true>()) : f(AttnCfg<T, true, 128, false>());
+    return rows ? f(AttnCfg<T, false, 128, true>()) : f(AttnCfg<T, false, 128, false>());
+  }
+  if (fp8) return rows ? f(AttnCfg<T, true, 64, true>()) : f(AttnCfg<T, true, 64, false>());
+  return rows ? f(AttnCfg<T, false, 64, true>()) : f(AttnCfg<T, false, 64, false>());
+}
+
 template <class T>
-static int launch_attn(const AttnArgs& a, int head_size, int dev, cudaStream_t st) {
-  // Rows of an average sequence: up to 16 the warps of a CTA split the tokens, beyond that the rows.
-  const bool rows = a.query_starts ? (long long)a.tokens * a.group > 16LL * a.seqs : a.group > 16;
+static int launch_attn(const AttnArgs& a, int head_size, void* workspace, size_t workspace_bytes, int dev, cudaStream_t st) {
   const bool fp8 = a.key_exp != nullptr;
-  // From 128 rows of an average sequence on the matrix products bound the call.
-  if ((long long)a.tokens * a.group >= 128LL * a.seqs && attn_tc_fits(a)) {
+  const AttnKind kind = attn_kind(a.tokens, a.seqs, a.group, a.query_starts == nullptr, attn_tc_fits(a));
+  if (kind == kAttnTensor) {
     if (head_size == 128) return fp8 ? launch_attn_tc<T, 128, true>(a, dev, st) : launch_attn_tc<T, 128, false>(a, dev, st);
     return fp8 ? launch_attn_tc<T, 64, true>(a, dev, st) : launch_attn_tc<T, 64, false>(a, dev, st);
   }
-#define TRB_ATTN(F, DD, R) return launch_attn<T, AttnCfg<T, F, DD, R>>(a, dev, st)
-  if (head_size == 128) {
-    if (fp8) { if (rows) TRB_ATTN(true, 128, true); else TRB_ATTN(true, 128, false); }
-    if (rows) TRB_ATTN(false, 128, true);
-    TRB_ATTN(false, 128, false);
-  }
-  if (fp8) { if (rows) TRB_ATTN(true, 64, true); else TRB_ATTN(true, 64, false); }
-  if (rows) TRB_ATTN(false, 64, true);
-  TRB_ATTN(false, 64, false);
-#undef TRB_ATTN
+  return attn_with_cfg<T>(fp8, head_size, kind == kAttnRows,
+                          [&](auto cfg) { return launch_attn<T, decltype(cfg)>(a, workspace, workspace_bytes, dev, st); });
 }
 
 }  // namespace trb
+
+extern "C" size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                                      int page_size, int table_width, int single, int e4m3, int dev) {
+  using namespace trb;
+  if (num_tokens <= 0 || num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || page_size <= 0 || table_width < 0)
+    return 0;
+  const int group = num_heads / num_kv_heads;
+  // The tensor-memory kernel needs none, but whether it takes the call also depends on the cache's strides.
+  const bool rows = attn_kind(num_tokens, num_seqs, group, single != 0, false) == kAttnRows;
+  return attn_with_cfg<__half>(e4m3 != 0, head_size, rows, [&](auto cfg) -> size_t {
+    using Cfg = decltype(cfg);
+    const int ctas = attn_cut<Cfg>(num_tokens, num_seqs, group, num_kv_heads, single != 0, (long long)table_width * page_size, sm_count(dev)).ctas;
+    return ctas > 1 ? 2ull * ctas * Cfg::PIECE_FLOATS * 4 : 0;
+  });
+}
 
 extern "C" int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
                                    const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,
@@ -36,7 +61,7 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
                                    long long query_head_stride, long long out_token_stride, long long out_head_stride,
                                    long long page_stride, long long token_stride, long long head_stride, long long exp_page_stride,
                                    long long exp_token_stride, long long exp_head_stride, float scale, int causal, int window, int dtype,
-                                   int dev, void* stream) {
+                                   void* workspace, size_t workspace_bytes, int dev, void* stream) {
   using namespace trb;
   if (num_tokens == 0 || num_seqs == 0) return TRB_OK;
   const bool fp8 = key_exponents != nullptr;
@@ -46,7 +71,7 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
   if (!query_starts && num_tokens != num_seqs) return TRB_ERR_BAD_ARG;
   if (num_heads % num_kv_heads != 0 || (window > 0 && !causal)) return TRB_ERR_PROB_SHAPE;
   const int esz = fp8 ? 1 : 2;
-  if (((uintptr_t)query | (uintptr_t)out | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15) return TRB_ERR_PROB_SHAPE;
+  if (((uintptr_t)query | (uintptr_t)out | (uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)workspace) & 15) return TRB_ERR_PROB_SHAPE;
   if ((query_token_stride | query_head_stride | out_token_stride | out_head_stride) & 7) return TRB_ERR_PROB_SHAPE;
   if (((page_stride | token_stride | head_stride) * esz) & 15) return TRB_ERR_PROB_SHAPE;
   // Positions are 32-bit numbers; the largest unit starts below length + 64.
@@ -62,6 +87,6 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
                    exp_head_stride, table_stride, num_pages, scale * 1.4426950408889634f, num_tokens, num_seqs, num_kv_heads,
                    num_heads / num_kv_heads, page_size, table_width,
                    (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1, causal, window};
-  if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, dev, (cudaStream_t)stream);
-  return launch_attn<__nv_bfloat16>(a, head_size, dev, (cudaStream_t)stream);
+  if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, workspace, workspace_bytes, dev, (cudaStream_t)stream);
+  return launch_attn<__nv_bfloat16>(a, head_size, workspace, workspace_bytes, dev, (cudaStream_t)stream);
 }

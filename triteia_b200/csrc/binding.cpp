@@ -227,11 +227,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     fresh = at::empty({T, heads, size}, query.options());
     out = &fresh;
   }
+  const int width = small(table.size(1), "page table's width");
+  // A buffer of each call's own: calls on different streams, and graphs that are replayed side by side, share nothing.
+  at::Tensor workspace;
+  const size_t bytes = trb_paged_attention_workspace_bytes(T, B, heads, c.heads, size, c.page_size, width, starts == nullptr, c.key_exp != nullptr, dev);
+  if (bytes > 0) workspace = at::empty({(int64_t)bytes}, query.options().dtype(at::kByte));
   const int status = trb_paged_attention(
       ptr(query), ptr(c.key), ptr(c.value), ptr(c.key_exp), ptr(c.value_exp), ptr(table), ptr(lengths), ptr(starts), out_ptr(*out), T, B,
-      heads, c.heads, size, c.page_size, c.pages, table.stride(0), small(table.size(1), "page table's width"), query.stride(0),
+      heads, c.heads, size, c.page_size, c.pages, table.stride(0), width, query.stride(0),
       query.stride(1), out->stride(0), out->stride(1), c.page, c.token, c.head, c.e_page, c.e_token, c.e_head, (float)scale, causal,
-      (int)(window > 0x7fffffff ? 0x7fffffff : window), tag, dev, stream_of(dev));
+      (int)(window > 0x7fffffff ? 0x7fffffff : window), tag,
+      bytes > 0 ? out_ptr(workspace) : nullptr, bytes, dev, stream_of(dev));
   check_status(status, "paged_attention", "heads of 64 or 128 that begin on 16-byte boundaries are needed");
   if (!fresh.defined()) return Py_NewRef(args[11]);
   return THPVariable_Wrap(std::move(fresh));
