@@ -227,7 +227,8 @@ int trb_rotary_embedding(const void* positions, void* query, void* key, const vo
  * num_kv_heads 0) have rows `*_stride` elements apart (multiples of 8, 16-byte aligned: parts of a fused q/k/v
  * product); query_out / key_out likewise, and may be the inputs.  Weights [head_size] of `dtype`, NULL: ones.
  * cos_sin_cache [max_position, rot_dim] of `dtype`, or of 32-bit floats with cache_is_f32; positions int64 [T]; a token
- * whose position is outside [0, max_position) is left alone (its output rows are not written).
+ * whose position is outside [0, max_position) is left alone (its output rows are not written).  eps < 0: no norm, the
+ * weights and the rotation alone.
  * head_size % 8 == 0, at most 256.  The reference has the rotation alone (csrc/ops/pos_encoding_kernels.cu:118-160). */
 int trb_qk_norm_rotary(const void* positions, const void* query, void* query_out, const void* key, void* key_out,
                        const void* query_weight, const void* key_weight, const void* cos_sin_cache, int cache_is_f32,

@@ -171,7 +171,7 @@ def test_what_is_no_tensor_is_a_type_error():
     (dict(head_size=0), "query must be"), (dict(query=Q[:2, :, ::2].flatten(1)[:, ::2]), "query must be"),
     (dict(cos_sin_cache=torch.zeros(8, 64, dtype=torch.float64)), "cos_sin_cache"), (dict(cos_sin_cache=torch.zeros(8, 128)[:, ::2]), "cos_sin_cache"),
     (dict(query_weight=torch.zeros(32, dtype=torch.float16)), "weight"), (dict(key_weight=torch.zeros(64)), "weight"),
-    (dict(query_out=Q.view(3, 256)), "query_out"), (dict(key_out=Q.view(3, 256)), "key_out"),
+    (dict(eps=-1e-6), "eps"), (dict(eps=float("nan")), "eps"), (dict(query_out=Q.view(3, 256)), "query_out"), (dict(key_out=Q.view(3, 256)), "key_out"),
 ])
 def test_norm_and_rotation_refuse_what_does_not_fit(change, what):
     a = dict(positions=torch.zeros(2, dtype=torch.int64), query=Q[:2].flatten(1).clone(), key=Q[:2].flatten(1).clone(), head_size=64,

@@ -594,3 +594,82 @@ def test_a_prompt_in_chunks_and_then_token_by_token(cuda, quantised):
             assert float(off.max()) <= 0
             at += n
     assert _lib.device_status(0) == 0
+
+
+@pytest.mark.parametrize("neox", [True, False])
+def test_rotation_without_a_norm(cuda, neox):
+    g = gen(31)
+    fused = normal(g, 37, 6 * 64 + 8)
+    q, k = fused[:, :256], fused[:, 256:384]
+    angle = torch.rand(50, 24, generator=g, device="cuda") * 6.28
+    table = torch.cat([angle.cos(), angle.sin()], 1).half()
+    pos = torch.randint(0, 50, (37,), generator=g, device="cuda")
+    w = (1 + 0.2 * normal(g, 64)).half()
+    for weight in (None, w):
+        qo, ko = torch.empty_like(q).contiguous(), torch.empty_like(k).contiguous()
+        capi.qk_norm_rotary_embedding(pos, q, k, 64, table, neox, weight, weight, None, qo, ko)
+        for x, got in ((q, qo), (k, ko)):
+            # the plain statement without its norm: scale the input so that the norm is one, and back
+            y = x.double().reshape(37, -1, 64)
+            n = (y.square().mean(-1, keepdim=True)).sqrt()
+            want, mag = plain_norm_rotary(pos, x, 64, table, neox, weight, 0.0)
+            want, mag = want * n.expand(-1, -1, 64).reshape(37, -1), mag * n.expand(-1, -1, 64).reshape(37, -1)
+            tol = U[torch.float16] * want.abs() + (1 + U[torch.float16]) * 80 * 2.0 ** -24 * mag + 2.0 ** -25
+            assert float(((got.double() - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("quantised,qk_norm", [(False, False), (True, True)])
+def test_delta_attention_block(cuda, quantised, qk_norm):
+    """The module runs its operators in order: a chunk of two sequences of different models and then a token of each, against the
+    same operators called one by one on a cache of their own and, between the projections, plain statements in 64 bits."""
+    from triteia_b200.nn import delta_attention
+
+    hidden, heads, kv_heads, size, D, page = 512, 4, 2, 128, 3, 16
+    m = delta_attention(hidden, heads, kv_heads, size, D, max_position=128, groupsize=128, qk_norm=qk_norm).to(cuda)
+    g = gen(60)
+    for name, k, n in (("qkv", hidden, 8 * size), ("o", heads * size, hidden)):
+        q, meta, s = ops.random_packed_deltas(D, k, n, groupsize=128, device=cuda, seed=1, scale_lo=0.002, scale_hi=0.004)
+        getattr(m, name + "_qweight").copy_(q), getattr(m, name + "_meta").copy_(meta), getattr(m, name + "_scale").copy_(s)
+        getattr(m, name + "_weight").copy_(normal(g, n, k) * k ** -0.5)
+    angle = torch.outer(torch.arange(128, device="cuda").double(), 10000.0 ** (-torch.arange(0, size, 2, device="cuda").double() / size))
+    m.cos_sin_cache.copy_(torch.cat([angle.cos(), angle.sin()], 1))
+    cache, own = (ops.new_cache(6, page, kv_heads, size, torch.float16, quantised) for _ in range(2))
+    table = torch.tensor([[4, 1, -1], [0, 3, 5]], dtype=torch.int32, device="cuda")
+    done, model = [0, 0], [2, -1]
+    history = [[], []]
+    for step in ([20, 33], [1, 1]):
+        T = sum(step)
+        x = normal(g, T, hidden)
+        pos = torch.cat([torch.arange(done[b], done[b] + step[b], device="cuda") for b in range(2)])
+        seq = torch.cat([torch.full((step[b],), b, device="cuda") for b in range(2)])
+        slots = table[seq, pos // page].long() * page + pos % page
+        idx = torch.tensor(model, dtype=torch.int32, device="cuda")[seq]
+        done = [done[b] + step[b] for b in range(2)]
+        lengths = torch.tensor(done, dtype=torch.int32, device="cuda")
+        starts = torch.tensor([0, step[0], T], dtype=torch.int32, device="cuda") if T > 2 else None
+        y = m(x, idx, pos, slots, cache, table, lengths, starts)
+        qkv = ops.sbmm_4bit_2_4_native(m.qkv_qweight, x, m.qkv_meta, m.qkv_scale, idx, base_weight=m.qkv_weight)
+        q, k, v = qkv.split([heads * size, kv_heads * size, kv_heads * size], 1)
+        capi.qk_norm_rotary_embedding(pos, q, k, size, m.cos_sin_cache, True, m.query_norm, m.key_norm, 1e-6 if qk_norm else None)
+        q, k, v = (t.unflatten(1, (-1, size)) for t in (q, k, v))
+        ops.cache_write(k, v, own[0], own[1], slots, own[2], own[3])
+        out = ops.paged_attention(q, own[0], own[1], table, lengths, starts, key_exponents=own[2], value_exponents=own[3])
+        assert torch.equal(y, ops.sbmm_4bit_2_4_native(m.o_qweight, out.flatten(1), m.o_meta, m.o_scale, idx, base_weight=m.o_weight))
+        at = 0
+        for b in range(2):
+            n = step[b]
+            new = [t[at:at + n].double() for t in (k, v)]
+            if quantised:
+                new = [c * torch.exp2(e)[..., None] for c, e in map(plain_codes, new)]
+            history[b].append(new)
+            keys, values = (torch.cat([h[i] for h in history[b]]) for i in range(2))
+            o, A, S = plain_attention(q[at:at + n], keys, values, done[b], n, size ** -0.5, True, None)
+            assert float(((out[at:at + n].double() - o).abs() - tolerance(o, A, S, done[b], torch.float16, quantised, size, float(values.abs().max()))).max()) <= 0
+            at += n
+
+
+def test_delta_attention_refuses_heads_that_do_not_divide(cuda):
+    from triteia_b200.nn import delta_attention
+
+    with pytest.raises(ValueError, match="key heads"):
+        delta_attention(512, 5, 2, 128, 1, 16)

@@ -15,7 +15,7 @@ def batched_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is
 
 def qk_norm_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight=None, key_weight=None,
                              eps=1e-6, query_out=None, key_out=None) -> None:
-    """The norm of every query and key head and the rotation in one pass (models with normed heads); in place, or into
-    query_out / key_out.  No counterpart in the reference."""
+    """The norm of every query and key head (eps=None: none) and the rotation in one pass, on rows that may be column ranges of a
+    fused projection; in place, or into query_out / key_out.  No counterpart in the reference."""
     triteia_cuda.qk_norm_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight, key_weight, eps,
                                           query_out, key_out)

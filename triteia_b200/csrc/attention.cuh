@@ -511,6 +511,8 @@ __device__ __forceinline__ T* attn_out_row(const AttnArgs& a, const AttnItem& it
   return static_cast<T*>(a.out) + (long long)(it.t.q0 + i) * a.o_tok + (long long)head * a.o_head;
 }
 
+constexpr int kAttnParts = 8;           // CTAs of a cluster at most
+
 // CLUSTER: a cluster shares one item (of a single-token call) instead, its CTAs' states meet through distributed shared memory,
 // and there is no line to cut and no second launch.
 template <class T, class Cfg, bool CLUSTER>
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     }
     cp_async_commit();
   };
-#pragma unroll
+#pragma unroll 1                        // fewer instructions to fetch: a short call meets each of them for the first time
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
   int slot = 0;
@@ -817,18 +819,29 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
         const uint32_t o_at = smem_base + Cfg::O_OFF, ml_at = smem_base + Cfg::ML_OFF;
         for (int x = (int)part * Cfg::THREADS + tid; x < t.rows * (D / 8); x += (int)parts * Cfg::THREADS) {
           const int row = x / (D / 8), d = (x % (D / 8)) * 8;
-          float m = -INFINITY, v[8] = {}, l = 0.f;
-          for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, ld_cluster_f32(mapa_shared(ml_at + row * 8, p)));
-          if (m != -INFINITY) {
-            for (uint32_t p = 0; p < parts; ++p) {
-              const float f_p = exp2_fast(ld_cluster_f32(mapa_shared(ml_at + row * 8, p)) - m);
-              l = fmaf(ld_cluster_f32(mapa_shared(ml_at + row * 8 + 4, p)), f_p, l);
-              const uint32_t src = mapa_shared(o_at + (row * Cfg::O_STRIDE + d) * 4, p);
-              const float4 w0 = ld_cluster_f32x4(src), w1 = ld_cluster_f32x4(src + 16);
-              const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          // Two round trips, whatever the number of neighbours: every load of one is in flight before the first is used.
+          float m = -INFINITY, v[8] = {}, l = 0.f, m_p[kAttnParts], l_p[kAttnParts];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = fmaf(w[e], f_p, v[e]);
-            }
+          for (int p = 0; p < kAttnParts; ++p) {
+            m_p[p] = p < parts ? ld_cluster_f32(mapa_shared(ml_at + row * 8, p)) : -INFINITY;
+            l_p[p] = p < parts ? ld_cluster_f32(mapa_shared(ml_at + row * 8 + 4, p)) : 0.f;
+          }
+          float4 w0[kAttnParts], w1[kAttnParts];
+#pragma unroll
+          for (int p = 0; p < kAttnParts; ++p) {
+            const uint32_t src = mapa_shared(o_at + (row * Cfg::O_STRIDE + d) * 4, p < parts ? p : 0);
+            w0[p] = ld_cluster_f32x4(src);
+            w1[p] = ld_cluster_f32x4(src + 16);
+          }
+#pragma unroll
+          for (int p = 0; p < kAttnParts; ++p) m = fmaxf(m, m_p[p]);
+#pragma unroll
+          for (int p = 0; p < kAttnParts; ++p) {
+            const float f_p = m_p[p] == -INFINITY ? 0.f : exp2_fast(m_p[p] - m);
+            l = fmaf(l_p[p], f_p, l);
+            const float w[8] = {w0[p].x, w0[p].y, w0[p].z, w0[p].w, w1[p].x, w1[p].y, w1[p].z, w1[p].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(w[e], f_p, v[e]);
           }
           attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
         }
@@ -920,7 +933,7 @@ static AttnCut attn_cut(long long tokens, int seqs, int group, int kv_heads, boo
   // and at most kShort for each CTA by the page table's width.
   constexpr int kShort = 8;
   if (single && !Cfg::ROWS && items * 2 <= slots) {
-    long long parts = slots / items < 8 ? slots / items : 8;
+    long long parts = slots / items < kAttnParts ? slots / items : kAttnParts;
     if (parts > (each + 1) / 2) parts = (each + 1) / 2;
     if (parts >= 1 && each <= kShort * parts) return {0, (int)parts, items};
   }

@@ -285,11 +285,13 @@ PyObject* qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       refuse("query_weight and key_weight must be contiguous [%d] tensors of query's dtype and device", size);
   if (positions.device() != query.device() || table.device() != query.device())
     refuse("positions and cos_sin_cache must be on the device of query");
+  const float eps = args[8] == Py_None ? 0.f : (float)real(args[8]);
+  if (!(eps >= 0.f)) refuse("eps must not be negative (None: no norm)");
   const int tag = tag_of(query.scalar_type()), dev = cuda_index(query);
   const int status = trb_qk_norm_rotary(
       ptr(positions), q.data, const_cast<void*>(q_out.data), k.data, const_cast<void*>(k_out.data), ptr(weights[0]), ptr(weights[1]),
       ptr(table), wide, table.size(0), small(q.rows, "number of tokens"), small(table.size(1), "rot_dim"), q.stride, q_out.stride, k.stride,
-      k_out.stride, (int)(q.cols / size), (int)(k.cols / size), size, (float)real(args[8]), truth(args[5]), tag, dev, stream_of(dev));
+      k_out.stride, (int)(q.cols / size), (int)(k.cols / size), size, args[8] == Py_None ? -1.f : eps, truth(args[5]), tag, dev, stream_of(dev));
   check_status(status, "qk_norm_rotary_embedding",
                "head_size is a multiple of 8 up to 256, rot_dim even and at most head_size, rows begin on 16-byte boundaries");
   Py_RETURN_NONE;

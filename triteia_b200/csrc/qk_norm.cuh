@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
-    const float r = rsqrtf(sum / (float)a.head_size + a.eps);
+    const float r = a.eps < 0.f ? 1.f : rsqrtf(sum / (float)a.head_size + a.eps);      // eps < 0: the rotation alone
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float p = PAIRS ? x[e ^ 1] : Ew<T>::to_f(t16[e]);

@@ -1,1 +1,2 @@
 from .linear import sparse_low_precision_linear
+from .attention import delta_attention

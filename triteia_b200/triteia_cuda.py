@@ -186,7 +186,7 @@ def batched_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is
 def qk_norm_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight=None, key_weight=None,
                              eps=1e-6, query_out=None, key_out=None):
     """Root-mean-square norm of every head of query and key (weights [head_size] or None), then rotary_embedding, one pass.
-    In place, or into query_out / key_out.  query [..., num_heads * head_size] and key [..., num_kv_heads * head_size] may be
+    eps=None: no norm, the weights and the rotation alone.  In place, or into query_out / key_out.  query [..., num_heads * head_size] and key [..., num_kv_heads * head_size] may be
     column ranges of a fused projection; cos_sin_cache [max_position, rot_dim] has query's dtype or float32.  A token whose
     position lies outside the cache is left alone."""
     _binding.qk_norm_rotary(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight, key_weight, eps, query_out, key_out)
