@@ -416,12 +416,19 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
   }
   if (need_mask) {
 #pragma unroll
-    for (int n = 0; n < 2 * NT; ++n)
+    for (int r = 0; r < 2; ++r) {
+      // Bit x: this row sees token j0 + x; then those of this lane's columns.
+      const int h = row_hi[r] - j0, w = row_lo[r] - j0;
+      unsigned long long bits = h >= 64 ? valid : h <= 0 ? 0ull : valid & ((1ull << h) - 1);
+      bits = w <= 0 ? bits : w >= 64 ? 0ull : bits & ~((1ull << w) - 1);
+      bits >>= 2 * quad;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int jl = n * 8 + 2 * quad + (e & 1), j = j0 + jl;
-        if (!((valid >> jl) & 1) || j >= row_hi[e >> 1] || j < row_lo[e >> 1]) s[n][e] = -INFINITY;
+      for (int n = 0; n < 2 * NT; ++n) {
+        const uint32_t two = (uint32_t)(bits >> (n * 8)) & 3;
+        if (!(two & 1)) s[n][2 * r] = -INFINITY;
+        if (!(two & 2)) s[n][2 * r + 1] = -INFINITY;
       }
+    }
   }
   // ---- running maxima
   float mx[2] = {st.m[0], st.m[1]};
@@ -624,7 +631,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
           }
         }
       } else {
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < WTOK / PER; ++i) {
           const int r = i * PER + r0;
           const long long ro = __shfl_sync(0xffffffffu, off, r) + c * 16;
@@ -637,10 +644,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     }
     cp_async_commit();
   };
-#pragma unroll 1                        // fewer instructions to fetch: a short call meets each of them for the first time
-  for (int i = 0; i < STAGES - 1; ++i) issue(i);
-
-  int slot = 0;
+  int slot = 0, warm = STAGES - 1;      // stage of the next unit; stages that are to be filled before it can be computed
   for (long long f = f0; f < f1 || CLUSTER;) {        // CLUSTER: one round, with nothing in it if the share is empty
     // ---- a piece: units [u, u_end) of item `it`
     int u = it.u0 + (int)(f - flat);
@@ -711,11 +715,19 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     const bool idle = wrow >= t.rows;
 
     f += u_end - u;
-    for (; u < u_end; ++u) {
-      cp_async_wait<STAGES - 2>();
-      if constexpr (Cfg::ROWS) __syncthreads();
-      else __syncwarp();
-      issue(slot == 0 ? STAGES - 1 : slot - 1);
+    // The loads are issued in one place, the first stages' too: the loop has to stay in the instruction cache, whose misses
+    // were the largest stall of this kernel while it held more.
+    while (u < u_end) {
+      if (warm == 0) {
+        cp_async_wait<STAGES - 2>();
+        if constexpr (Cfg::ROWS) __syncthreads();
+        else __syncwarp();
+      }
+      issue(warm > 0 ? STAGES - 1 - warm : slot == 0 ? STAGES - 1 : slot - 1);
+      if (warm > 0) {
+        --warm;
+        continue;
+      }
       if (!idle) {
         constexpr int TOK = Cfg::NT * 16;
         const int own = Cfg::ROWS ? 0 : warp * WTOK;
@@ -733,6 +745,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
       }
       if constexpr (!Cfg::ROWS) __syncwarp();
       slot = slot + 1 == STAGES ? 0 : slot + 1;
+      ++u;
     }
 
     // ---- the piece's state: to the output, or to the workspace (slot 2 c of CTA c for the item its run begins in, or with;
