@@ -241,7 +241,7 @@ int trb_qk_norm_rotary(const void* positions, const void* query, void* query_out
  * elements, multiples of 8); slots int64 [T], slot = page * page_size + place.  Exponents NULL: the cache holds `dtype`.
  * Else it holds e4m3 codes and for every (token, head) an exponent byte b (strides exp_*), value = code * 2^(b - 127):
  * b - 127 is the smallest integer e with max |x| <= 448 * 2^e over the finite values of the head (0 for a head of zeros,
- * never below -126), codes are rounded to nearest even, infinities and NaN become NaN.
+ * never below -126), codes are rounded to nearest even, infinities and NaN become NaN.  A byte of 255 stands for no number.
  *   trb_cache_write  a token whose slot is outside [0, num_pages * page_size) is skipped (padding); each slot at most
  *                    once in a call (of two tokens with one slot, parts of either may be stored)
  *   trb_cache_read   key_out / value_out [T, heads, head_size] contiguous of `dtype`; zeros for a slot outside the cache
@@ -269,8 +269,9 @@ int trb_cache_read(const void* key_cache, const void* value_cache, const void* k
  *   out = sum_j softmax_j(scale * q . k_j) v_j, zero where nothing is seen; query head h reads key head
  *   h / (num_heads / num_kv_heads).
  * A page outside [0, num_pages) counts as masked; a length beyond table_width * page_size counts as that.  Rows of out
- * outside every sequence are not written.  What lies in the cache at or beyond a sequence's length is never used; keys and
- * values below it are expected to be finite numbers.
+ * outside every sequence are not written.  What lies in the cache at or beyond a sequence's length, or before the window of
+ * all its new tokens, is never used; keys and values of the other tokens are finite numbers (a NaN or an infinity among them
+ * may reach every new token of its sequence).
  * query and out [T, num_heads, head_size] of `dtype` with strides that are multiples of 8; head_size 64 or 128.
  * Stands for the programs of triteia/triton/decode_attention.py:30-214 and extend_attention.py:39-170. */
 int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,

@@ -165,6 +165,7 @@ DECODE = ([1, 0, 16, 17, 255, 1000, 63, 64, 65], [1] * 9)
 CHUNKS = ([5, 40, 300, 0, 129, 64, 77], [5, 3, 130, 0, 1, 64, 76])
 SHORT = ([3, 0, 70, 33], [7, 4, 2, 40])            # more new tokens than the cache has: the first see nothing
 LONG = ([700, 1500], [300, 515])
+LONG_SHORT = ([300, 100, 0], [400, 150, 200])      # the same in calls that the matrix products bound
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -182,7 +183,7 @@ def test_attention(cuda, dtype, e4m3, heads, kv_heads, size, page, plan):
 
 @pytest.mark.parametrize("dtype,e4m3", [(torch.float16, False), (torch.bfloat16, False), (torch.bfloat16, True)])
 @pytest.mark.parametrize("causal,window", [(False, None), (True, 1), (True, 16), (True, 100), (True, 5000)])
-@pytest.mark.parametrize("plan", [DECODE, CHUNKS, SHORT, LONG], ids=["decode", "chunks", "short", "long"])
+@pytest.mark.parametrize("plan", [DECODE, CHUNKS, SHORT, LONG, LONG_SHORT], ids=["decode", "chunks", "short", "long", "long-short"])
 def test_attention_masks(cuda, dtype, e4m3, causal, window, plan):
     b = Batch(2, *plan, 8, 2, 128, 16, dtype, e4m3)
     b.check(b.call(causal=causal, window=window), causal=causal, window=window)
@@ -345,6 +346,65 @@ def test_attention_in_a_cache_beyond_32_bit_offsets(cuda, e4m3, new):
             setattr(small, name, e)
     small.table = table
     small.check(small.call())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [1, 300])
+def test_attention_where_a_stride_says_nothing(cuda, e4m3, new):
+    """One key head, one page, one query head, one token: dimensions of one entry, with strides of no use."""
+    b = Batch(16, [32], [min(new, 32)], 1, 1, 64, 32, torch.float16, e4m3)
+    page = int(b.table[0, 0])
+    b.table[0, 0] = 0
+
+    def odd(x):
+        return x[page:page + 1].as_strided((1, 32, 1, 64), (7, 64, 5, 1), x[page:page + 1].storage_offset())
+
+    def odd_exps(x):
+        return None if x is None else x[page:page + 1].as_strided((1, 32, 1), (3, 1, 9), x[page:page + 1].storage_offset())
+
+    b.kc, b.vc, b.ke, b.ve = odd(b.kc), odd(b.vc), odd_exps(b.ke), odd_exps(b.ve)
+    T = b.q.shape[0]
+    b.q = b.q.as_strided((T, 1, 64), (11 if T == 1 else 64, 13, 1))
+    b.check(b.call())
+    if new == 1:
+        b.starts = None
+        b.check(b.call())
+    slots = torch.arange(32, device="cuda")
+    k, v = ops.cache_read(b.kc, b.vc, slots, b.ke, b.ve, dtype=torch.float16)
+    again = (b.kc.clone(), b.vc.clone(), None if b.ke is None else b.ke.clone(), None if b.ve is None else b.ve.clone())
+    ops.cache_write(k.as_strided((32, 1, 64), (64, 3, 1)), v, again[0], again[1], slots, again[2], again[3])
+    assert torch.equal(torch.stack(ops.cache_read(again[0], again[1], slots, again[2], again[3], dtype=torch.float16)), torch.stack((k, v)))
+
+
+@pytest.mark.parametrize("new", [1, 3, 200])
+def test_attention_without_pages(cuda, new):
+    """Sequences whose table has no columns: nothing is seen."""
+    kc, vc, _, _ = ops.new_cache(2, 16, 2, 64)
+    q = normal(gen(17), 2 * new, 4, 64)
+    out = ops.paged_attention(q, kc, vc, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), torch.full((2,), 50, dtype=torch.int32, device="cuda"),
+                              torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda"))
+    assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (96, 1), (200, 1), (17, 1)])
+def test_attention_of_many_heads_over_one(cuda, e4m3, heads, kv_heads):
+    for plan in (([100, 0, 33], [1, 1, 1]), ([100, 40], [7, 12]), ([200, 300], [30, 1])):
+        b = Batch(18, *plan, heads, kv_heads, 64, 16, torch.bfloat16, e4m3)
+        b.check(b.call())
+        if sum(plan[1]) == len(plan[1]):
+            b.starts = None
+            b.check(b.call())
+
+
+def test_attention_of_more_sequences_than_a_warp_has_lanes(cuda):
+    lengths = [(37 * i) % 150 for i in range(70)]
+    for new in ([1] * 70, [(i % 5) * 3 for i in range(70)]):
+        b = Batch(19, lengths, new, 8, 2, 64, 16, torch.float16, False)
+        b.check(b.call())
+        if new == [1] * 70:
+            b.starts = None
+            b.check(b.call())
 
 
 @pytest.mark.parametrize("e4m3", [False, True])

@@ -69,6 +69,12 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
       num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0) || window < 0)
     return TRB_ERR_BAD_ARG;
   if (!query_starts && num_tokens != num_seqs) return TRB_ERR_BAD_ARG;
+  // The stride of a dimension of one entry says nothing.
+  if (num_kv_heads == 1) head_stride = head_size;
+  if (page_size == 1) token_stride = head_size;
+  if (num_pages == 1) page_stride = head_size;
+  if (num_tokens == 1) query_token_stride = out_token_stride = 0;
+  if (num_heads == 1) query_head_stride = out_head_stride = 0;
   if (num_heads % num_kv_heads != 0 || (window > 0 && !causal)) return TRB_ERR_PROB_SHAPE;
   const int esz = fp8 ? 1 : 2;
   if (((uintptr_t)query | (uintptr_t)out | (uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)workspace) & 15) return TRB_ERR_PROB_SHAPE;

@@ -222,7 +222,12 @@ static int launch_kv(const KvArgs& a, bool fp8, bool write, int dtype, int dev, 
   return cudaGetLastError() == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
 }
 
-static int kv_check(const KvArgs& a, long long num_pages, bool fp8) {
+static int kv_check(KvArgs& a, long long num_pages, bool fp8) {
+  // The stride of a dimension of one entry says nothing.
+  if (a.heads == 1) a.c_head = a.k_head = a.v_head = 0;
+  if (a.page_size == 1) a.c_tok = 0;
+  if (num_pages == 1) a.c_page = 0;
+  if (a.tokens == 1) a.k_tok = a.v_tok = 0;
   if (a.tokens < 0 || a.heads <= 0 || num_pages < 0 || a.page_size <= 0) return TRB_ERR_BAD_ARG;
   if (a.head_size <= 0 || a.head_size % 8 != 0 || a.head_size > 256) return TRB_ERR_PROB_SHAPE;
   const uintptr_t cache_align = fp8 ? 7 : 15;
@@ -242,13 +247,12 @@ extern "C" int trb_cache_write(const void* key, const void* value, const void* s
   if (num_tokens == 0) return TRB_OK;
   const bool fp8 = key_exponents != nullptr;
   if (!key || !value || !slots || !key_cache || !value_cache || fp8 != (value_exponents != nullptr)) return TRB_ERR_BAD_ARG;
-  const KvArgs a{key, value, nullptr, nullptr, key_cache, value_cache, (uint8_t*)key_exponents, (uint8_t*)value_exponents,
+  KvArgs a{key, value, nullptr, nullptr, key_cache, value_cache, (uint8_t*)key_exponents, (uint8_t*)value_exponents,
                  (const int64_t*)slots, num_pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride,
                  page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride, exp_head_stride, num_tokens, heads,
                  head_size, page_size};
   if (const int err = kv_check(a, num_pages, fp8)) return err;
-  if (((uintptr_t)key | (uintptr_t)value) & 15 || ((key_token_stride | key_head_stride | value_token_stride | value_head_stride) & 7))
-    return TRB_ERR_PROB_SHAPE;
+  if (((uintptr_t)key | (uintptr_t)value) & 15 || ((a.k_tok | a.k_head | a.v_tok | a.v_head) & 7)) return TRB_ERR_PROB_SHAPE;
   if (dtype != TRB_F16 && dtype != TRB_BF16) return TRB_ERR_KERN_SHAPE;
   return launch_kv(a, fp8, true, dtype, dev, (cudaStream_t)stream);
 }
@@ -262,7 +266,7 @@ extern "C" int trb_cache_read(const void* key_cache, const void* value_cache, co
   if (num_tokens == 0) return TRB_OK;
   const bool fp8 = key_exponents != nullptr;
   if (!key_out || !value_out || !slots || !key_cache || !value_cache || fp8 != (value_exponents != nullptr)) return TRB_ERR_BAD_ARG;
-  const KvArgs a{nullptr, nullptr, key_out, value_out, const_cast<void*>(key_cache), const_cast<void*>(value_cache),
+  KvArgs a{nullptr, nullptr, key_out, value_out, const_cast<void*>(key_cache), const_cast<void*>(value_cache),
                  (uint8_t*)key_exponents, (uint8_t*)value_exponents, (const int64_t*)slots, num_pages * page_size, 0, 0, 0, 0,
                  page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride, exp_head_stride, num_tokens, heads,
                  head_size, page_size};

@@ -216,6 +216,7 @@ extern "C" int trb_qk_norm_rotary(const void* positions, const void* query, void
     return TRB_ERR_BAD_ARG;
   if (head_size <= 0 || head_size % 8 != 0 || head_size > 256 || rot_dim < 0 || rot_dim % 2 != 0 || rot_dim > head_size)
     return TRB_ERR_PROB_SHAPE;
+  if (num_tokens == 1) query_stride = query_out_stride = key_stride = key_out_stride = 0;      // of one row: says nothing
   if (((uintptr_t)query | (uintptr_t)query_out) & 15 || ((query_stride | query_out_stride) & 7) != 0) return TRB_ERR_PROB_SHAPE;
   if (num_kv_heads > 0 && (((uintptr_t)key | (uintptr_t)key_out) & 15 || ((key_stride | key_out_stride) & 7) != 0)) return TRB_ERR_PROB_SHAPE;
   if (dtype != TRB_F16 && dtype != TRB_BF16) return TRB_ERR_KERN_SHAPE;

@@ -15,6 +15,10 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_st
     (int32 [B + 1]; None: one new token per sequence).  A new token at position p sees the positions up to p (causal; all of
     the sequence otherwise), the last `window` of them where a window is given; a row that sees nothing is zero.  heads is a
     multiple of the cache's heads.  Rows of out that belong to no sequence are left as they are; a negative page counts as
-    masked.  scale: 1 / sqrt(head_size) by default."""
+    masked.  scale: 1 / sqrt(head_size) by default.
+
+    What lies in the cache at or beyond a sequence's length, or before the window of all its new tokens, is never used.  Keys and
+    values of the other tokens are finite numbers: a NaN or an infinity among them may reach every new token of its sequence,
+    also those that do not see it."""
     return _binding.paged_attention(query, key_cache, value_cache, page_table, lengths, query_starts, scale, causal, window, key_exponents,
                                     value_exponents, out)
