@@ -543,6 +543,13 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     skip = (int)((uint32_t)it.n * part / parts);
     f0 = skip;
     f1 = (uint32_t)it.n * (part + 1) / parts;
+  } else if (pieces == nullptr) {       // a CTA for each item
+    if (!attn_find_tile<M>(a, blockIdx.x / a.kv_heads, it.t)) return;
+    it.kvh = blockIdx.x % a.kv_heads;
+    attn_item_units<M, UNIT>(a, it);
+    skip = 0;
+    f0 = 0;
+    f1 = it.n;
   } else {
     pdl_launch_dependents();            // the joining launch waits for this one's end before it reads
     long long own;
@@ -929,7 +936,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
   attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
 }
 
-// How a call is cut.  ctas > 0: runs of the line, one wave of two CTAs per SM.  parts > 0: clusters of that many.
+// How a call is cut.  ctas > 0: runs of the line, one wave of two CTAs per SM.  parts > 0: clusters of that many.  Neither: a
+// CTA for each item.
 struct AttnCut {
   int ctas, parts;
   long long items;
@@ -950,6 +958,9 @@ static AttnCut attn_cut(long long tokens, int seqs, int group, int kv_heads, boo
     if (parts > (each + 1) / 2) parts = (each + 1) / 2;
     if (parts >= 1 && each <= kShort * parts) return {0, (int)parts, items};
   }
+  // Short items that are resident at once: nothing to even out, and neither the scan of the batch nor the second launch
+  // (8 sequences of 101 tokens, 8 heads, e4m3: 18.7 us with them).
+  if (each <= kShort && items <= slots) return {0, 0, items};
   const long long ctas = items * each / 2 < slots ? items * each / 2 : slots;
   return {ctas < 1 ? 1 : (int)ctas, 0, items};
 }
@@ -978,10 +989,11 @@ static int launch_attn(const AttnArgs& a, void* workspace, size_t workspace_byte
   }
   static std::atomic<bool> done[64];
   if (!ensure_smem_attr(attn_kernel<T, Cfg, false>, dev, Cfg::SMEM_BYTES, done)) return TRB_ERR_CUDA;
-  if (cut.ctas > 1 && (workspace == nullptr || workspace_bytes < 2ull * cut.ctas * Cfg::PIECE_FLOATS * 4)) return TRB_ERR_SCRATCH;
-  attn_kernel<T, Cfg, false><<<cut.ctas, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a, (float*)workspace);
+  const bool line = cut.ctas > 0;
+  if (line && (workspace == nullptr || workspace_bytes < 2ull * cut.ctas * Cfg::PIECE_FLOATS * 4)) return TRB_ERR_SCRATCH;
+  attn_kernel<T, Cfg, false><<<line ? cut.ctas : (int)cut.items, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a, line ? (float*)workspace : nullptr);
   if (cudaGetLastError() != cudaSuccess) return TRB_ERR_CUDA;
-  if (cut.ctas == 1) return TRB_OK;
+  if (cut.ctas <= 1) return TRB_OK;
   cfg.gridDim = dim3(cut.ctas - 1, Cfg::M * (Cfg::D / 8) / 128);
   cfg.blockDim = dim3(128);
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

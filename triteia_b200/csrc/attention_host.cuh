@@ -50,7 +50,7 @@ extern "C" size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_se
   return attn_with_cfg<__half>(e4m3 != 0, head_size, rows, [&](auto cfg) -> size_t {
     using Cfg = decltype(cfg);
     const int ctas = attn_cut<Cfg>(num_tokens, num_seqs, group, num_kv_heads, single != 0, (long long)table_width * page_size, sm_count(dev)).ctas;
-    return ctas > 1 ? 2ull * ctas * Cfg::PIECE_FLOATS * 4 : 0;
+    return 2ull * ctas * Cfg::PIECE_FLOATS * 4;
   });
 }
 
