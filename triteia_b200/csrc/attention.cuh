@@ -889,10 +889,14 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
 }
 
 // Joins the pieces of the items that a border of two CTAs' runs cuts; `ctas`: the grid of the launch before.  CTA (c, y) has
-// part y of the item that the end of run c cuts first.
+// every gridDim.y-th group of the (row, 8 sizes) cells of the item that the end of run c cuts first.  Few pieces: a thread
+// for each cell.  Many (a long sequence has up to one for every CTA): 32 cells at a time, and eight warps share the pieces, so
+// that they are read in a few round trips; their states meet in a fixed order.
+constexpr int kJoinWarps = 8;
 template <class T, class Cfg>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const float* pieces, int ctas) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs a, const float* pieces, int ctas) {
   constexpr int D = Cfg::D, M = Cfg::M, UNIT = Cfg::UNIT;
+  __shared__ float states[kJoinWarps][10][32];
   long long own;
   const long long total = attn_total_units<M, UNIT>(a, own);
   const int c = blockIdx.x;
@@ -904,36 +908,69 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
   pdl_wait();                                         // the pieces are there; and this launch never ends before that one
   const long long s = border - at, e = s + it.n;
   if (at == 0 || runs.begin(c) > s) return;                // nothing is cut here, or an earlier border cuts it too
-  const int x = blockIdx.y * 128 + threadIdx.x;
-  if (x >= it.t.rows * (D / 8)) return;
-  const int row = x / (D / 8), d = (x % (D / 8)) * 8;
   // Pieces of CTAs c .. c + n - 1; an empty run (fewer units than CTAs) has none.
   int n = 1;
   while (runs.begin(c + n) < e) ++n;
   const float* first = pieces + (2LL * c + (runs.begin(c) < s ? 1 : 0)) * Cfg::PIECE_FLOATS;
   const float* rest = pieces + 2LL * c * Cfg::PIECE_FLOATS;
-  auto piece_of = [&](int k) { return k == 0 ? first : rest + 2LL * k * Cfg::PIECE_FLOATS; };
-  auto held = [&](int k) { return runs.each > 0 || runs.begin(c + k + 1) > runs.begin(c + k); };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int k = 0; k < n; ++k)
-    if (held(k)) m = fmaxf(m, piece_of(k)[M * D + 2 * row]);
-  float v[8] = {}, l = 0.f;
-  if (m != -INFINITY) {
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      if (!held(k)) continue;
-      const float* p = piece_of(k);
-      const float2 ml = *reinterpret_cast<const float2*>(p + M * D + 2 * row);
-      const float4 v0 = *reinterpret_cast<const float4*>(p + row * D + d), v1 = *reinterpret_cast<const float4*>(p + row * D + d + 4);
-      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-      l = fmaf(ml.y, f, l);
-      const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool shared = n > 4;            // the warps share the pieces of a cell
+  const int cells = it.t.rows * (D / 8), step = shared ? 32 : kJoinWarps * 32;
+  for (int x0 = blockIdx.y * step; x0 < cells; x0 += gridDim.y * step) {
+    const int x = x0 + (shared ? lane : (int)threadIdx.x);
+    const bool on = x < cells;
+    const int row = on ? x / (D / 8) : 0, d = (x % (D / 8)) * 8;
+    float m = -INFINITY, l = 0.f, v[8] = {};
+    // One state into the running one.
+    auto add = [&](float m2, float l2, const float (&w)[8]) {
+      const float top = fmaxf(m, m2);
+      const float f = m == -INFINITY ? 0.f : exp2_fast(m - top), g = m2 == -INFINITY ? 0.f : exp2_fast(m2 - top);
+      m = top;
+      l = fmaf(l, f, l2 * g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(w[i], f, v[i]);
+      for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], f, w[i] * g);
+    };
+    constexpr int AHEAD = 4;            // pieces whose loads are in flight together
+    const int stride = shared ? kJoinWarps : 1;
+    for (int k0 = shared ? warp : 0; k0 < n; k0 += stride * AHEAD) {
+      float2 ml[AHEAD];
+      float4 v0[AHEAD], v1[AHEAD];
+#pragma unroll
+      for (int y = 0; y < AHEAD; ++y) {
+        const int k = k0 + y * stride;
+        ml[y] = make_float2(-INFINITY, 0.f);
+        v0[y] = v1[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on && k < n && (runs.each > 0 || runs.begin(c + k + 1) > runs.begin(c + k))) {
+          const float* p = k == 0 ? first : rest + 2LL * k * Cfg::PIECE_FLOATS;
+          ml[y] = *reinterpret_cast<const float2*>(p + M * D + 2 * row);
+          v0[y] = *reinterpret_cast<const float4*>(p + row * D + d);
+          v1[y] = *reinterpret_cast<const float4*>(p + row * D + d + 4);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < AHEAD; ++y) {
+        const float w[8] = {v0[y].x, v0[y].y, v0[y].z, v0[y].w, v1[y].x, v1[y].y, v1[y].z, v1[y].w};
+        add(ml[y].x, ml[y].y, w);
+      }
     }
+    if (shared) {
+      states[warp][0][lane] = m;
+      states[warp][1][lane] = l;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) states[warp][2 + i][lane] = v[i];
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kJoinWarps; ++w) {
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = states[w][2 + i][lane];
+          add(states[w][0][lane], states[w][1][lane], z);
+        }
+      }
+    }
+    if (on && (warp == 0 || !shared)) attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
+    if (shared) __syncthreads();        // before the next cells' states
   }
-  attn_store_row<T, 8>(attn_out_row<T>(a, it, row) + d, v, l);
 }
 
 // How a call is cut.  ctas > 0: runs of the line, one wave of two CTAs per SM.  parts > 0: clusters of that many.  Neither: a
@@ -994,8 +1031,8 @@ static int launch_attn(const AttnArgs& a, void* workspace, size_t workspace_byte
   attn_kernel<T, Cfg, false><<<line ? cut.ctas : (int)cut.items, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a, line ? (float*)workspace : nullptr);
   if (cudaGetLastError() != cudaSuccess) return TRB_ERR_CUDA;
   if (cut.ctas <= 1) return TRB_OK;
-  cfg.gridDim = dim3(cut.ctas - 1, Cfg::M * (Cfg::D / 8) / 128);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(cut.ctas - 1, Cfg::ROWS ? 4 : 1);
+  cfg.blockDim = dim3(kJoinWarps * 32);
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   return cudaLaunchKernelEx(&cfg, attn_join_kernel<T, Cfg>, a, (const float*)workspace, cut.ctas) == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
