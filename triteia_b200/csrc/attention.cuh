@@ -995,9 +995,9 @@ static AttnCut attn_cut(long long tokens, int seqs, int group, int kv_heads, boo
     if (parts > (each + 1) / 2) parts = (each + 1) / 2;
     if (parts >= 1 && each <= kShort * parts) return {0, (int)parts, items};
   }
-  // Short items that are resident at once: nothing to even out, and neither the scan of the batch nor the second launch
-  // (8 sequences of 101 tokens, 8 heads, e4m3: 18.7 us with them).
-  if (each <= kShort && items <= slots) return {0, 0, items};
+  // Short items, a few waves of them at most: nothing to even out, and neither the scan of the batch nor the second launch
+  // (8 sequences of 101 tokens, 8 heads, e4m3: 18.7 us with them, 10.0 without; 27 of 61 tokens, 32 heads: 20.4 and 12).
+  if (each <= kShort && items <= 4 * slots) return {0, 0, items};
   const long long ctas = items * each / 2 < slots ? items * each / 2 : slots;
   return {ctas < 1 ? 1 : (int)ctas, 0, items};
 }
