@@ -54,25 +54,38 @@ __device__ __forceinline__ void kv_store(uint4 raw, unsigned lanes, bool active,
   if constexpr (!FP8) {
     if (active) *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at) = raw;
   } else {
-    const T* e16 = reinterpret_cast<const T*>(&raw);
-    float x[8], top = 0.f;
+    // Magnitudes compare like the integers that their bits are, two at a time.
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t most = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = Ew<T>::to_f(e16[e]);
-      const float m = fabsf(x[e]);
-      if (m <= 3.402823466e38f) top = fmaxf(top, m);
-      else x[e] = __uint_as_float(0x7fffffffu);
+    for (int e = 0; e < 4; ++e) most = __vmaxu2(most, word[e] & 0x7fff7fffu);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(lanes, most, o));
+    most = max(most & 0xffffu, most >> 16);
+    float2 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = two_of(word[e], T());
+    float top = two_of(most, T()).x;
+    if (most >= kInf) {                                 // infinities or NaN in the head: the largest of the others
+      top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mx = fabsf(x[e].x), my = fabsf(x[e].y);
+        if (mx <= 3.402823466e38f) top = fmaxf(top, mx);
+        else x[e].x = __uint_as_float(0x7fffffffu);
+        if (my <= 3.402823466e38f) top = fmaxf(top, my);
+        else x[e].y = __uint_as_float(0x7fffffffu);
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
     }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
     const int byte = kv_exponent_byte(top);
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);      // 2^-(byte - 127): byte is 1 .. 247
     uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float2 p = make_float2(x[e] * inv, x[e + 1] * inv);
-      w[e >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(p, __NV_SATFINITE, __NV_E4M3) << (8 * (e & 3));
-    }
+    for (int e = 0; e < 4; ++e)
+      w[e >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(mul2(x[e], make_float2(inv, inv)), __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
     if (active) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at) = make_uint2(w[0], w[1]);
     if (first) *byte_out = (uint8_t)byte;
   }

@@ -28,6 +28,42 @@ struct DeviceGuard {
   }
 };
 
+// Two 32-bit products, sums or multiply-adds in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+// The two numbers of a word.
+__device__ __forceinline__ float2 two_of(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 two_of(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t word_of(float2 v, __half) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t word_of(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 struct QkNormArgs {
   const int64_t* positions;
   const void *query, *key;            // key may be null (num_kv_heads 0 then)
@@ -127,6 +163,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
     }
   }
   if (!there) return;
+  const float inv_size = 1.f / (float)a.head_size;
 #pragma unroll
   for (int u = 0; u < kQkHeads; ++u) {
     const int h = h0 + u * step;
@@ -151,21 +188,23 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
       }
       __syncwarp(lanes);
     }
-    T* e16 = reinterpret_cast<T*>(&raw[u]);
-    const T* t16 = reinterpret_cast<const T*>(&them);
-    float x[8], sum = 0.f;
+    uint32_t* mine = reinterpret_cast<uint32_t*>(&raw[u]);
+    const uint32_t* theirs = reinterpret_cast<const uint32_t*>(&them);
+    float2 x[4], sum2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = Ew<T>::to_f(e16[e]);
-      sum = fmaf(x[e], x[e], sum);
+    for (int e = 0; e < 4; ++e) {
+      x[e] = two_of(mine[e], T());
+      sum2 = fma2(x[e], x[e], sum2);
     }
+    float sum = sum2.x + sum2.y;
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
-    const float r = a.eps < 0.f ? 1.f : rsqrtf(sum / (float)a.head_size + a.eps);      // eps < 0: the rotation alone
+    const float r = a.eps < 0.f ? 1.f : rsqrtf(sum * inv_size + a.eps);      // eps < 0: the rotation alone
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = PAIRS ? x[e ^ 1] : Ew<T>::to_f(t16[e]);
-      e16[e] = Ew<T>::from_f(fmaf(x[e], own[e], p * other[e]) * r);
+    for (int e = 0; e < 4; ++e) {
+      const float2 p = PAIRS ? make_float2(x[e].y, x[e].x) : two_of(theirs[e], T());
+      const float2 y = fma2(x[e], make_float2(own[2 * e], own[2 * e + 1]), mul2(p, make_float2(other[2 * e], other[2 * e + 1])));
+      mine[e] = word_of(mul2(y, make_float2(r, r)), T());
     }
     if (active) *reinterpret_cast<uint4*>(out + (long long)h * a.head_size + d0) = raw[u];
   }
