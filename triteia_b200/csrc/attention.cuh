@@ -19,6 +19,10 @@
 // borders.  An item inside a run is finished there; of one that a border cuts, the pieces' states (maximum, sum, weighted
 // values) go to the caller's workspace, and a second launch joins them in the order of the tokens: no counters, nothing to
 // clear, a fixed order of the sums.
+// Measured: 64 sequences of 100 to 8000 tokens, 32 heads over 8 of 128, bf16: 161 us, 6.0 TB/s of the 6.55 that a copy reaches;
+// three of 90000 to 131072 tokens, e4m3: 132 us, 5.1 TB/s -- there the conversions make the loop longer than the instruction
+// cache takes well (two of three stalled cycles wait for instructions).  Clusters for all calls (one launch, no workspace)
+// left half of the SMs idle with twelve CTAs each and unequal sequences unequal: 184 and 197 us.
 // Loads are 16-byte cp.async with a row address per token (any page size and strides); a token outside the visible range
 // or on a page outside the cache is filled with zeros and masked.
 #pragma once

@@ -7,7 +7,8 @@
 // A group of G = head_size / 8 lanes (rounded up to a power of two) holds one head, 8 elements = 16 bytes a lane: the sum of
 // squares is log2(G) shuffles, a NeoX partner's inputs come with four more.  A group has up to five heads of ONE token and
 // asks for all of them, for the position and then for its cosines and sines at once, so that a CTA waits for memory twice and
-// no more: with loops over the heads of a token (fewer and longer CTAs) 8191 x 80 heads took 80 to 90 us, now 61 (5.5 TB/s; four heads a group 74, eight 74).
+// no more: with loops over the heads of a token (fewer and longer CTAs) 8191 x 80 heads took 80 to 90 us, now 57.5 (5.9 TB/s;
+// before the arithmetic went two numbers at a time 61 with five heads a group, 74 with four or eight).
 #pragma once
 
 #include "elementwise.cuh"
