@@ -324,6 +324,40 @@ def test_attention_gives_the_same_bits_again_in_graphs_and_on_other_streams(cuda
     assert torch.equal(on_side, want) and torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want_c)
 
 
+@pytest.mark.parametrize("plan", [DECODE, CHUNKS, ([900, 40, 2000], [1, 1, 1])], ids=["decode", "chunks", "long-decode"])
+def test_attention_calls_side_by_side_on_two_streams(cuda, plan):
+    batches = [Batch(70 + i, *plan, 8, 2, 128, 16, torch.float16, i == 1) for i in range(2)]
+    want = [b.call().clone() for b in batches]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in batches], [[], []]
+    for _ in range(20):
+        for i, b in enumerate(batches):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(b.call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+def test_attention_refuses_a_workspace_that_is_too_small(cuda):
+    b = Batch(20, [5000, 3000], [1, 1], 8, 2, 128, 16, torch.float16, False)
+    out = torch.full_like(b.q, 5)
+    need = _lib.lib.trb_paged_attention_workspace_bytes(2, 2, 8, 2, 128, 16, b.table.shape[1], 1, 0, 0)
+    assert need > 0
+    room = torch.empty(need, dtype=torch.uint8, device="cuda")
+
+    def call(workspace, nbytes):
+        s = b.kc.stride()
+        return _lib.lib.trb_paged_attention(
+            _lib.ptr(b.q), _lib.ptr(b.kc), _lib.ptr(b.vc), None, None, _lib.ptr(b.table), _lib.ptr(b.len), None, _lib.ptr(out), 2, 2, 8, 2, 128, 16,
+            b.kc.shape[0], b.table.stride(0), b.table.shape[1], b.q.stride(0), b.q.stride(1), out.stride(0), out.stride(1), s[0], s[1], s[2], 0, 0, 0,
+            128 ** -0.5, 1, 0, 0, workspace, nbytes, 0, _lib.stream_of(b.q))
+
+    assert call(None, 0) == _lib.ERR_SCRATCH and call(_lib.ptr(room), need - 16) == _lib.ERR_SCRATCH
+    assert bool((out == 5).all())
+    assert call(_lib.ptr(room), need) == _lib.TRB_OK
+    b.check(out)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("new", [1, 9, 260])
 def test_attention_in_a_cache_beyond_32_bit_offsets(cuda, e4m3, new):
