@@ -51,7 +51,7 @@ def build_binding(force=False):
            + [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                                  os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
            + [BINDING_SRC, "-o", BINDING, f"-L{PKG}", "-ltriteia_b200", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",
-              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+              "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

@@ -792,51 +792,93 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
       float* obuf = reinterpret_cast<float*>(smem + Cfg::O_OFF);
       float2* ml = reinterpret_cast<float2*>(smem + Cfg::ML_OFF);
       float2* wml = reinterpret_cast<float2*>(smem + Cfg::WML_OFF);
-      if (quad == 0) {
-        wml[warp * 16 + (lane >> 2)] = make_float2(st.m[0], st.l[0]);
-        wml[warp * 16 + (lane >> 2) + 8] = make_float2(st.m[1], st.l[1]);
-      }
-      __syncthreads();
-      float f_row[2];
+      if constexpr (CLUSTER) {
+        // No loads are under way: the warps' states go to the ring side by side and are added in one pass (a short call
+        // feels every barrier).
+        cp_async_wait<0>();
+        __syncthreads();
+        float* wbuf = reinterpret_cast<float*>(smem) + warp * 16 * Cfg::O_STRIDE;
 #pragma unroll
-      for (int rr = 0; rr < 2; ++rr) {
-        const int row = (lane >> 2) + 8 * rr;
-        float m = -INFINITY, l = 0.f;
+        for (int rr = 0; rr < 2; ++rr) {
+          const int row = (lane >> 2) + 8 * rr;
+          if (row >= t.rows) continue;
+          if (quad == 0) wml[warp * 16 + row] = make_float2(st.m[rr], st.l[rr]);
+          float* dst = wbuf + row * Cfg::O_STRIDE;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, wml[w * 16 + row].x);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float2 s = wml[w * 16 + row];
-          if (s.x != -INFINITY) l = fmaf(s.y, exp2_fast(s.x - m), l);
-        }
-        f_row[rr] = st.m[rr] == -INFINITY ? 0.f : exp2_fast(st.m[rr] - m);
-        if (warp == 0 && quad == 0) ml[row] = make_float2(m, l);
-      }
-      // The warps add their parts one after the other: a fixed order.
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (warp == w) {
-#pragma unroll
-          for (int rr = 0; rr < 2; ++rr) {
-            float* dst = obuf + ((lane >> 2) + 8 * rr) * Cfg::O_STRIDE;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              // Sizes 4 quad .. + 3 of each 16 (e4m3), or 2 quad, + 1 of each 8.
-              float4 v = Cfg::FP8 ? make_float4(st.o[2 * d][2 * rr], st.o[2 * d + 1][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr + 1])
-                                  : make_float4(st.o[2 * d][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr], st.o[2 * d + 1][2 * rr + 1]);
-              v = make_float4(v.x * f_row[rr], v.y * f_row[rr], v.z * f_row[rr], v.w * f_row[rr]);
-              float2* p0 = reinterpret_cast<float2*>(dst + d * 16 + (Cfg::FP8 ? 4 : 2) * quad);
-              float2* p1 = Cfg::FP8 ? p0 + 1 : p0 + 4;
-              if (w > 0) {
-                v.x += p0->x, v.y += p0->y;
-                v.z += p1->x, v.w += p1->y;
-              }
-              *p0 = make_float2(v.x, v.y);
-              *p1 = make_float2(v.z, v.w);
-            }
+          for (int d = 0; d < D / 16; ++d) {
+            // Sizes 4 quad .. + 3 of each 16 (e4m3), or 2 quad, + 1 of each 8.
+            float2* p0 = reinterpret_cast<float2*>(dst + d * 16 + (Cfg::FP8 ? 4 : 2) * quad);
+            float2* p1 = Cfg::FP8 ? p0 + 1 : p0 + 4;
+            *p0 = Cfg::FP8 ? make_float2(st.o[2 * d][2 * rr], st.o[2 * d + 1][2 * rr]) : make_float2(st.o[2 * d][2 * rr], st.o[2 * d][2 * rr + 1]);
+            *p1 = Cfg::FP8 ? make_float2(st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr + 1])
+                           : make_float2(st.o[2 * d + 1][2 * rr], st.o[2 * d + 1][2 * rr + 1]);
           }
         }
         __syncthreads();
+        for (int x = tid; x < t.rows * (D / 4); x += Cfg::THREADS) {
+          const int row = x / (D / 4), d = (x % (D / 4)) * 4;
+          float m = -INFINITY, l = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) m = fmaxf(m, wml[w * 16 + row].x);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float2 ws = wml[w * 16 + row];
+            const float f_w = ws.x == -INFINITY ? 0.f : exp2_fast(ws.x - m);
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + (w * 16 + row) * Cfg::O_STRIDE + d);
+            l = fmaf(ws.y, f_w, l);
+            o = make_float4(fmaf(v.x, f_w, o.x), fmaf(v.y, f_w, o.y), fmaf(v.z, f_w, o.z), fmaf(v.w, f_w, o.w));
+          }
+          *reinterpret_cast<float4*>(obuf + row * Cfg::O_STRIDE + d) = o;
+          if (d == 0) ml[row] = make_float2(m, l);
+        }
+      } else {
+        if (quad == 0) {
+          wml[warp * 16 + (lane >> 2)] = make_float2(st.m[0], st.l[0]);
+          wml[warp * 16 + (lane >> 2) + 8] = make_float2(st.m[1], st.l[1]);
+        }
+        __syncthreads();
+        float f_row[2];
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+          const int row = (lane >> 2) + 8 * rr;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) m = fmaxf(m, wml[w * 16 + row].x);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float2 s = wml[w * 16 + row];
+            if (s.x != -INFINITY) l = fmaf(s.y, exp2_fast(s.x - m), l);
+          }
+          f_row[rr] = st.m[rr] == -INFINITY ? 0.f : exp2_fast(st.m[rr] - m);
+          if (warp == 0 && quad == 0) ml[row] = make_float2(m, l);
+        }
+        // The warps add their parts one after the other: a fixed order.
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (warp == w) {
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              float* dst = obuf + ((lane >> 2) + 8 * rr) * Cfg::O_STRIDE;
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) {
+                // Sizes 4 quad .. + 3 of each 16 (e4m3), or 2 quad, + 1 of each 8.
+                float4 v = Cfg::FP8 ? make_float4(st.o[2 * d][2 * rr], st.o[2 * d + 1][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr + 1])
+                                    : make_float4(st.o[2 * d][2 * rr], st.o[2 * d][2 * rr + 1], st.o[2 * d + 1][2 * rr], st.o[2 * d + 1][2 * rr + 1]);
+                v = make_float4(v.x * f_row[rr], v.y * f_row[rr], v.z * f_row[rr], v.w * f_row[rr]);
+                float2* p0 = reinterpret_cast<float2*>(dst + d * 16 + (Cfg::FP8 ? 4 : 2) * quad);
+                float2* p1 = Cfg::FP8 ? p0 + 1 : p0 + 4;
+                if (w > 0) {
+                  v.x += p0->x, v.y += p0->y;
+                  v.z += p1->x, v.w += p1->y;
+                }
+                *p0 = make_float2(v.x, v.y);
+                *p1 = make_float2(v.z, v.w);
+              }
+            }
+          }
+          __syncthreads();
+        }
       }
       if constexpr (CLUSTER) {
         cluster_sync_all();

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -86,6 +87,11 @@ int cuda_index(const at::Tensor& t) {
 }
 
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+
+// A new tensor, past the dispatcher (half a microsecond a tensor).
+at::Tensor fresh_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
 
 bool last_contiguous(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1; }
 
@@ -180,7 +186,7 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   check_vector(slots, "slots", at::kLong, slots.numel(), device);
   const int T = small(slots.numel(), "number of tokens");
   const int dev = cuda_index(kc);
-  at::Tensor key = at::empty({T, c.heads, c.size}, kc.options().dtype(type)), value = at::empty({T, c.heads, c.size}, kc.options().dtype(type));
+  at::Tensor key = fresh_tensor({T, c.heads, c.size}, type, device), value = fresh_tensor({T, c.heads, c.size}, type, device);
   const int status = trb_cache_read(ptr(c.key), ptr(c.value), ptr(c.key_exp), ptr(c.value_exp), ptr(slots), out_ptr(key), out_ptr(value), T,
                                     c.heads, c.size, c.page_size, c.pages, c.page, c.token, c.head, c.e_page, c.e_token, c.e_head, tag, dev,
                                     stream_of(dev));
@@ -224,14 +230,14 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     refuse("out must have the shape, dtype and device of query and a contiguous last dimension");
   const int tag = tag_of(query.scalar_type()), dev = cuda_index(query);
   if (!out) {
-    fresh = at::empty({T, heads, size}, query.options());
+    fresh = fresh_tensor({T, heads, size}, query.scalar_type(), device);
     out = &fresh;
   }
   const int width = small(table.size(1), "page table's width");
   // A buffer of each call's own: calls on different streams, and graphs that are replayed side by side, share nothing.
   at::Tensor workspace;
   const size_t bytes = trb_paged_attention_workspace_bytes(T, B, heads, c.heads, size, c.page_size, width, starts == nullptr, c.key_exp != nullptr, dev);
-  if (bytes > 0) workspace = at::empty({(int64_t)bytes}, query.options().dtype(at::kByte));
+  if (bytes > 0) workspace = fresh_tensor({(int64_t)bytes}, at::kByte, device);
   const int status = trb_paged_attention(
       ptr(query), ptr(c.key), ptr(c.value), ptr(c.key_exp), ptr(c.value_exp), ptr(table), ptr(lengths), ptr(starts), out_ptr(*out), T, B,
       heads, c.heads, size, c.page_size, c.pages, table.stride(0), width, query.stride(0),
