@@ -476,31 +476,33 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     {
       const T* qp = static_cast<const T*>(a.query) + (long long)(t.q0 + qi) * a.q_tok + (long long)head * a.q_head;
       const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-      float up = 1.f;
+      // The whole row on its way before the first store, which no load may pass.
+      uint4 w[D / 8];
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x) w[x] = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
       if constexpr (!std::is_same<T, TM>::value) {    // bf16 as fp16: see AttnMma
         float top = 0.f;
 #pragma unroll
         for (int x = 0; x < D / 8; ++x) {
-          const uint4 w = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
-          const T* e = reinterpret_cast<const T*>(&w);
+          const uint32_t word[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
 #pragma unroll
-          for (int y = 0; y < 8; ++y) top = fmaxf(top, fabsf(Ew<T>::to_f(e[y])));
+          for (int y = 0; y < 4; ++y) {
+            const float2 v = two_of(word[y], T());
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
         }
         const int k = attn_row_shift(top);
-        up = __uint_as_float((uint32_t)k << 23);
+        const float up = __uint_as_float((uint32_t)k << 23);
         c *= __uint_as_float((uint32_t)(254 - k) << 23);
+        auto scaled = [&](uint32_t word) { return word_of(mul2(two_of(word, T()), make_float2(up, up)), TM()); };
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) w[x] = make_uint4(scaled(w[x].x), scaled(w[x].y), scaled(w[x].z), scaled(w[x].w));
       }
 #pragma unroll
       for (int x = 0; x < D / 8; ++x) {
-        uint4 w = on ? *reinterpret_cast<const uint4*>(qp + x * 8) : make_uint4(0, 0, 0, 0);
-        if constexpr (!std::is_same<T, TM>::value) {
-          const T* e = reinterpret_cast<const T*>(&w);
-          const uint32_t h[4] = {pack2(Ew<T>::to_f(e[0]) * up, Ew<T>::to_f(e[1]) * up, TM()), pack2(Ew<T>::to_f(e[2]) * up, Ew<T>::to_f(e[3]) * up, TM()),
-                                 pack2(Ew<T>::to_f(e[4]) * up, Ew<T>::to_f(e[5]) * up, TM()), pack2(Ew<T>::to_f(e[6]) * up, Ew<T>::to_f(e[7]) * up, TM())};
-          w = make_uint4(h[0], h[1], h[2], h[3]);
-        }
         const uint32_t at = qtile + (x >> 3) * 16384 + row * 128 + (((x & 7) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x ^ flip), "r"(w.y ^ flip), "r"(w.z ^ flip), "r"(w.w ^ flip)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[x].x ^ flip), "r"(w[x].y ^ flip), "r"(w[x].z ^ flip),
+                     "r"(w[x].w ^ flip)
                      : "memory");
       }
       fence_proxy_async();
@@ -707,11 +709,19 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     __syncwarp();
     const long long out_at = on ? (long long)(t.q0 + qi) * a.o_tok + (long long)head * a.o_head : -1;
     constexpr int CH = D / 8;                         // 16-byte pieces of a row
-#pragma unroll 4
-    for (int x = 0; x < CH; ++x) {
-      const int r = x * (32 / CH) + lane / CH, ch = lane % CH;
-      const long long at = __shfl_sync(0xffffffffu, out_at, r);
-      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + ch * 8) = lds128(patch + attn_swizzle<D * 2>(r, ch));
+#pragma unroll
+    for (int x0 = 0; x0 < CH; x0 += 4) {
+      uint4 w[4];
+      long long at[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = (x0 + x) * (32 / CH) + lane / CH;
+        at[x] = __shfl_sync(0xffffffffu, out_at, r);
+        w[x] = lds128(patch + attn_swizzle<D * 2>(r, lane % CH));
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (at[x] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at[x] + (lane % CH) * 8) = w[x];
     }
   }
   tc_fence_before();
