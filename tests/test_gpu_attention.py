@@ -447,6 +447,19 @@ def test_attention_far_into_a_document(cuda, e4m3):
     b.check(b.call())
 
 
+@pytest.mark.parametrize("dtype,e4m3", [(torch.float16, False), (torch.bfloat16, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("causal,window", [(False, None), (True, None), (True, 100)])
+@pytest.mark.parametrize("heads,kv_heads,size,page", [(8, 2, 128, 16), (40, 20, 128, 24), (80, 40, 64, 64)])
+@pytest.mark.parametrize("lengths,new", [([3000], [60]), ([2900, 0, 1200], [70, 0, 40]), ([2500, 200], [64, 200]), ([1700], [300])],
+                         ids=["one", "three", "uneven", "wide"])
+def test_attention_of_few_tokens_over_many(cuda, dtype, e4m3, causal, window, heads, kv_heads, size, page, lengths, new):
+    b = Batch(16, lengths, new, heads, kv_heads, size, page, dtype, e4m3)
+    out = b.call(causal=causal, window=window)
+    b.check(out, causal=causal, window=window)
+    for _ in range(3):
+        assert same(out, b.call(causal=causal, window=window))
+
+
 # ------------------------------------------------------------------------------------------------ cache
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("quantised", [False, True])

@@ -22,13 +22,17 @@
 // powers of two enter at the scores, as in attention.cuh: 2^(t_j - m) with t_j = log2 weight + e_j meets the code of v_j.
 // Queries and weights are fp16 there whatever T is (queries scaled by a power of two per row).
 //
-// Measured (32 heads of 128): a prompt of 8192 tokens over 32 key heads, fp16, 520 us = 1.06 PFLOP/s (610 us in a loop, where
-// the power cap holds the clock at 1.64 GHz); five chunks of 20 to 700 tokens over 1020 to 6000, 8 key heads, bf16, 152 us; two
-// chunks over 8362 and 12000 e4m3 tokens 309 us.  A key tile takes a CTA about 3400 clocks, of which the MMAs need 2048 and the
-// exponentials as many (16 a clock); the rest is the way of one tile from its scores to the next ones.  Calls with few items
-// lose most to the last wave: cutting them like the short calls (persistent CTAs, pieces joined) cost 8 us a piece and was
-// slower (152 -> 190 us).  Moving a quarter or half of the exponentials to the multiply-add pipe changed the chunks by -2 and
-// +1 %, the prompt by +1 and +6 %.
+// A call with few items over long keys gives each item to a cluster of 2, 4 or 8 CTAs, which walk a run of its key tiles each
+// and join their states over distributed shared memory; the rule and its figures stand at the launch.
+//
+// Measured (32 heads of 128): a prompt of 8192 tokens over 32 key heads, fp16, 516 us = 1.07 PFLOP/s (605 us in a loop, where
+// the power cap holds the clock at 1.64 GHz); five chunks of 20 to 700 tokens over 1020 to 6000, 8 key heads, bf16, 145 us; two
+// chunks over 8362 and 12000 e4m3 tokens 301 us.  A key tile takes a CTA about 3400 clocks, of which the MMAs need 2048 and the
+// exponentials as many (16 a clock); the rest is the way of one tile from its scores to the next ones.  Calls of one to a few
+// waves lose most to the last one.  Cutting them like the short calls (persistent CTAs, pieces joined) cost 8 us a piece and was
+// slower (152 -> 190 us); so were clusters of two where they do not all run at once (chunks 144 -> 152, e4m3 300 -> 307).
+// Moving a quarter or half of the exponentials to the multiply-add pipe changed the chunks by -2 and +1 %, the prompt by +1 and
+// +6 %.
 //
 // Shared memory: 64 KB of queries and a ring of five 32 KB tiles (K0, V0, K1, ..) -- e4m3: three, and three of codes.
 // 512 tensor memory columns: S and O of both tiles.
@@ -133,10 +137,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-template <class T, class Cfg>
+// SPLIT: the 2, 4 or 8 CTAs of a cluster share an item, each with a run of its key tiles.  At the end CTA r finishes the rows of
+// 8 / split softmax warps: the others send it those rows' outputs, maxima and sums, through distributed shared memory into its
+// idle ring.
+template <class T, class Cfg, bool SPLIT>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a, int tiles_bound,
-               int box) {
+               int box, int split) {
   using TM = typename AttnMma<T, Cfg::FP8>::type;
   constexpr int D = Cfg::D, BUFS = Cfg::BUFS, CODE_BUFS = Cfg::CODE_BUFS;
   extern __shared__ uint8_t smem_raw[];
@@ -157,13 +164,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // Late tiles of a causal prompt see the most keys: they go first.
-  const int kvh = blockIdx.x % a.kv_heads;
+  const int item = SPLIT ? blockIdx.x / split : blockIdx.x, rank = SPLIT ? blockIdx.x % split : 0;
+  const int kvh = item % a.kv_heads;
   AttnTile t;
-  if (!attn_find_tile<256>(a, tiles_bound - 1 - (int)(blockIdx.x / a.kv_heads), t)) return;
+  if (!attn_find_tile<256>(a, tiles_bound - 1 - item / a.kv_heads, t)) return;
   int lo, hi;
   attn_key_range(a, t, lo, hi);
-  // Key tiles [kt0, kt0 + n[i]) concern the rows of tile i.
-  const int kt0 = lo / 128;
+  // Key tiles [kt0, kt0 + n[i]) of this CTA concern the rows of tile i.
+  const int all = hi > lo ? (hi + 127) / 128 - lo / 128 : 0;
+  const int k0 = SPLIT ? (int)((long long)all * rank / split) : 0, k1 = SPLIT ? (int)((long long)all * (rank + 1) / split) : all;
+  const int kt0 = lo / 128 + k0;
   const int base_pos = t.length - t.new_tokens;
   int n[2];
 #pragma unroll
@@ -173,7 +183,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     if (a.causal && rows > 0) h = min(hi, base_pos + (t.row0 + 128 * i + rows - 1) / a.group + 1);
     // The same in every lane, which the reduction tells the compiler: loop counters and the MMAs' operands stay in uniform
     // registers.
-    n[i] = __reduce_max_sync(0xffffffffu, rows > 0 && h > lo ? (h + 127) / 128 - kt0 : 0);
+    n[i] = __reduce_max_sync(0xffffffffu, rows > 0 && h > lo ? max(0, min((h + 127) / 128 - lo / 128, k1) - k0) : 0);
   }
   const int n_all = max(n[0], n[1]);
 
@@ -398,6 +408,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       ask_pages(i + 2);
     }
    }
+   if constexpr (SPLIT) {
+     __syncwarp();
+     cluster_sync_all();
+     cluster_sync_all();
+   }
   } else if (warp >= 12) {
     // ------------------------------ e4m3: codes -> fp16 tiles ------------------------------
     if constexpr (Cfg::FP8) {
@@ -459,6 +474,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           if (++buf == BUFS) { buf = 0; phase ^= 1; }
         }
         if (lane == 0) mbar_arrive(&fac_free[i & 1]);
+      }
+      if constexpr (SPLIT) {
+        __syncwarp();
+        cluster_sync_all();
+        cluster_sync_all();
       }
     }
   } else {
@@ -683,6 +703,48 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     } else {
       mbar_wait(q_bar, 0, dead);                      // the staging rows below are the queries' rows
     }
+    // SPLIT: the ring takes [sender][row] of float [D + 4], then as many pairs of maximum and sum.
+    constexpr int kRow = (D + 4) * 4;
+    static_assert(224 * (kRow + 8) <= Cfg::EXP_OFF - Cfg::KV_OFF);
+    const int share = SPLIT ? 8 / split : 8, owner = (tile * 4 + quarter) / share;
+    const int sent = share * 32, at_row = (tile * 4 + quarter) % share * 32 + lane;       // rows per sender, this row among them
+    const uint32_t in_o = smem_base + Cfg::KV_OFF, in_ml = in_o + (SPLIT ? (split - 1) * sent * kRow : 0);
+    float f_own = 1.f;
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_sync_all();                             // every MMA of every CTA has retired, so no load is under way: the rings are idle
+      if (owner != rank) {
+        const int slot = (rank - (rank > owner)) * sent + at_row;
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+          uint32_t o[32] = {};
+          if (n[tile] > 0) {
+            tc_ld32(o_addr + b * 32, o);
+            tc_wait_ld32(o);
+          }
+          const uint32_t to = mapa_shared(in_o + slot * kRow + b * 128, owner);
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) st_cluster_v4(to + x * 4, o[x], o[x + 1], o[x + 2], o[x + 3]);
+        }
+        const uint32_t to = mapa_shared(in_ml + slot * 8, owner);
+        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(__float_as_uint(m)), "r"(__float_as_uint(l)) : "memory");
+      }
+      __syncwarp();
+      cluster_sync_all();
+      if (owner == rank) {
+        float top = m;
+        for (int s = 0; s < split - 1; ++s) top = fmaxf(top, __uint_as_float(lds32(in_ml + (s * sent + at_row) * 8)));
+        f_own = m == -INFINITY ? 0.f : exp2_fast(m - top);
+        l *= f_own;
+        for (int s = 0; s < split - 1; ++s) {
+          const uint32_t at = in_ml + (s * sent + at_row) * 8;
+          const float m2 = __uint_as_float(lds32(at)), f = m2 == -INFINITY ? 0.f : exp2_fast(m2 - top);
+          l = fmaf(__uint_as_float(lds32(at + 4)), f, l);
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "f"(f) : "memory");   // only this thread reads it
+        }
+      }
+    }
+    if (!SPLIT || owner == rank) {
     // Every MMA of this tile has retired: its queries' rows take the output on its way to whole rows in memory.
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const uint32_t patch = qtile + quarter * (32 * D * 2);
@@ -692,6 +754,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       if (n[tile] > 0) {
         tc_ld32(o_addr + b * 32, o);
         tc_wait_ld32(o);
+      }
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f_own);
+        for (int s = 0; s < split - 1; ++s) {
+          const float f = __uint_as_float(lds32(in_ml + (s * sent + at_row) * 8));
+          const uint32_t from = in_o + (s * sent + at_row) * kRow + b * 128;
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            const uint4 z = lds128(from + x * 4);
+            o[x] = __float_as_uint(fmaf(__uint_as_float(z.x), f, __uint_as_float(o[x])));
+            o[x + 1] = __float_as_uint(fmaf(__uint_as_float(z.y), f, __uint_as_float(o[x + 1])));
+            o[x + 2] = __float_as_uint(fmaf(__uint_as_float(z.z), f, __uint_as_float(o[x + 2])));
+            o[x + 3] = __float_as_uint(fmaf(__uint_as_float(z.w), f, __uint_as_float(o[x + 3])));
+          }
+        }
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -722,6 +800,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         if (at[x] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at[x] + (lane % CH) * 8) = w[x];
+    }
     }
   }
   tc_fence_before();
@@ -766,19 +845,50 @@ static bool attn_tc_fits(const AttnArgs& a) {
 template <class T, int D, bool FP8>
 static int launch_attn_tc(const AttnArgs& a, int dev, cudaStream_t st) {
   using Cfg = AttnTcCfg<D, FP8>;
-  static std::atomic<bool> done[64];
-  if (!ensure_smem_attr(attn_tc_kernel<T, Cfg>, dev, Cfg::SMEM_ALLOC, done)) return TRB_ERR_CUDA;
   const int box = attn_tc_box(a.page_size);
   CUtensorMap tk, tv;
   constexpr CUtensorMapDataType type = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                        : std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (!make_map_cache(&tk, type, a.key_cache, a, D, box) || !make_map_cache(&tv, type, a.value_cache, a, D, box)) return TRB_ERR_CUDA;
   const long long per_token = (a.group + 255) / 256;
-  long long tiles = (long long)a.tokens * a.group / 256 + a.seqs;
+  long long tiles = ((long long)a.tokens * a.group + 255LL * a.seqs) / 256;      // every sequence's last tile may hold one row
   if (tiles > a.tokens * per_token) tiles = a.tokens * per_token;
   const long long grid = tiles * a.kv_heads;
-  if (grid > 0x7fffffffLL) return TRB_ERR_PROB_SHAPE;
-  attn_tc_kernel<T, Cfg><<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM_ALLOC, st>>>(tk, tv, a, (int)tiles, box);
+  if (grid > 0x3fffffffLL) return TRB_ERR_PROB_SHAPE;
+  // Few items over long keys: the largest cluster per item with which all clusters still run at once, two key tiles or more per
+  // CTA, by the page table's width.  Below 8 key tiles sending the states costs more than it saves (32 heads over 8 of size 128,
+  // bf16, one CTA -> a cluster: 128 tokens after 500: 18.5 -> 19.8 us; after 1000: 25.1 -> 23.0; after 2000: 38 -> 26.5; 64 tokens
+  // after 8000: 116 -> 34.7; 256 after 4000: 65 -> 35.7; 512 after 4000: 65 -> 47).
+  const long long key_tiles = ((long long)a.table_width * a.page_size + 127) / 128;
+  for (int split = 8; split >= 2; split /= 2) {
+    if (grid * split > sm_count(dev) || key_tiles < (split == 8 ? 16 : 8)) continue;
+    static std::atomic<bool> shared[64];
+    static std::atomic<int> fit[64][4];               // clusters that run at once
+    if (!ensure_smem_attr(attn_tc_kernel<T, Cfg, true>, dev, Cfg::SMEM_ALLOC, shared)) return TRB_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(grid * split));
+    cfg.blockDim = dim3(Cfg::THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM_ALLOC;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    std::atomic<int>& most = fit[dev < 64 ? dev : 0][split == 8 ? 3 : split / 2];
+    int n = dev < 64 ? most.load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<T, Cfg, true>, &cfg) != cudaSuccess) return TRB_ERR_CUDA;
+      most.store(n > 0 ? n : -1, std::memory_order_relaxed);
+    }
+    if (grid > n) continue;
+    return cudaLaunchKernelEx(&cfg, attn_tc_kernel<T, Cfg, true>, tk, tv, a, (int)tiles, box, split) == cudaSuccess ? TRB_OK
+                                                                                                                    : TRB_ERR_CUDA;
+  }
+  static std::atomic<bool> done[64];
+  if (!ensure_smem_attr(attn_tc_kernel<T, Cfg, false>, dev, Cfg::SMEM_ALLOC, done)) return TRB_ERR_CUDA;
+  attn_tc_kernel<T, Cfg, false><<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM_ALLOC, st>>>(tk, tv, a, (int)tiles, box, 1);
   return cudaGetLastError() == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
 }
 
