@@ -189,6 +189,15 @@ def test_attention_masks(cuda, dtype, e4m3, causal, window, plan):
     b.check(b.call(causal=causal, window=window), causal=causal, window=window)
 
 
+@pytest.mark.parametrize("dtype,e4m3", [(torch.float16, False), (torch.bfloat16, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("causal,window", [(False, None), (True, None), (True, 16), (True, 100)])
+@pytest.mark.parametrize("size,page", [(128, 8), (64, 40)])
+@pytest.mark.parametrize("plan", [CHUNKS, SHORT, LONG], ids=["chunks", "short", "long"])
+def test_attention_masks_over_small_pages(cuda, dtype, e4m3, causal, window, size, page, plan):
+    b = Batch(17, *plan, 8, 2, size, page, dtype, e4m3)
+    b.check(b.call(causal=causal, window=window), causal=causal, window=window)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_attention_scale(cuda, scale):
     b = Batch(3, *CHUNKS, 8, 4, 64, 16, torch.float16, False)

@@ -8,7 +8,7 @@
 //
 // A work tile is M rows of one sequence and one key head; a row is a (token, query head of the group), so that the g
 // heads of a group share every key and value that is read.  This kernel serves the calls that reading the cache bounds
-// (single tokens, short chunks) and the caches that the tensor-memory kernel does not take.  Per 16 x 16 block of scores it
+// (single and few tokens) and the caches that the tensor-memory kernel does not take.  Per 16 x 16 block of scores it
 // issues two m16n8k16 MMAs for each 16 of the head size, one running maximum per row, and as many MMAs again with the
 // values.
 //   M = 16: the four warps of a CTA take different tokens (16 each of every 64) and keep softmax states of their own,

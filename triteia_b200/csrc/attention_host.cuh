@@ -5,13 +5,17 @@
 
 namespace trb {
 
-// Which kernel takes a call.  From 128 rows (token, query head of a group) of an average sequence on the matrix products
-// bound it; up to 16 rows the warps of a CTA split the tokens, beyond that the rows.
+// Which kernel takes a call, by the rows (token, query head of a group) of an average sequence: up to 16 the warps of a CTA split
+// the tokens; more go to the tensor-memory kernel where its page and stride rules hold, and else to CTAs whose warps split the
+// rows.  Tensor memory against split rows, bf16, heads 32 over 8 of size 128: 8 tokens of one sequence after 8000: 28.8 and 34.6
+// us, 24 of each of 32 after 2000: 64 and 118, 700 after 800 next to 127 single ones after 1000: 150 and 228; 6 of each of 200
+// after 900: 217 and 221, of size 64 e4m3 122 and 112, its worst.  Below 17 rows splitting the tokens wins (4 of each of 128 after
+// 1000: 134 and 103).
 enum AttnKind { kAttnSplit, kAttnRows, kAttnTensor };
 static AttnKind attn_kind(long long tokens, int seqs, int group, bool single, bool tensor_fits) {
   const long long rows = single ? (long long)group * seqs : tokens * group;
-  if (!single && rows >= 128LL * seqs && tensor_fits) return kAttnTensor;
-  return rows > 16LL * seqs ? kAttnRows : kAttnSplit;
+  if (rows <= 16LL * seqs) return kAttnSplit;
+  return !single && tensor_fits ? kAttnTensor : kAttnRows;
 }
 
 // Calls f with the configuration of the kernel for short calls.
