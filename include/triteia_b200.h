@@ -241,7 +241,8 @@ int trb_qk_norm_rotary(const void* positions, const void* query, void* query_out
  * elements, multiples of 8); slots int64 [T], slot = page * page_size + place.  Exponents NULL: the cache holds `dtype`.
  * Else it holds e4m3 codes and for every (token, head) an exponent byte b (strides exp_*), value = code * 2^(b - 127):
  * b - 127 is the smallest integer e with max |x| <= 448 * 2^e over the finite values of the head (0 for a head of zeros,
- * never below -126), codes are rounded to nearest even, infinities and NaN become NaN.  A byte of 255 stands for no number.
+ * never below -126), codes are rounded to nearest even, infinities and NaN become NaN.  A byte of 255 stands for no number;
+ * a head of zeros has the byte 127 also where others fill the cache (attention knows it by that).
  *   trb_cache_write  a token whose slot is outside [0, num_pages * page_size) is skipped (padding); each slot at most
  *                    once in a call (of two tokens with one slot, parts of either may be stored)
  *   trb_cache_read   key_out / value_out [T, heads, head_size] contiguous of `dtype`; zeros for a slot outside the cache

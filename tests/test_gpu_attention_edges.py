@@ -1,0 +1,73 @@
+"""GPU: attention where a cache, a mask or a batch is unusual.  Statements and tolerances as in test_gpu_attention.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import LONG_SHORT, SHORT, Batch, gen, normal, plain_attention, tolerance
+from triteia_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def check(b, out, scale=None, vmax=None, causal=True, window=None):
+    """Batch.check with the largest value that has weight (vmax) given: one that has none must not widen the tolerance."""
+    size, at = b.q.shape[2], 0
+    scale = size ** -0.5 if scale is None else scale
+    for i, (length, n) in enumerate(zip(b.lengths, b.new)):
+        k, v = b.tokens(i)
+        o, A, S = plain_attention(b.q[at:at + n], k, v, length, n, scale, causal, window)
+        got = out[at:at + n].double()
+        assert torch.isfinite(got).all(), f"sequence {i}: not finite"
+        most = float(v.abs().max()) if vmax is None else vmax
+        off = (got - o).abs() - tolerance(o, A, S, length, b.dtype, b.e4m3, size, most)
+        assert float(off.max()) <= 0, f"sequence {i} ({n} of {length}): {float(off.max())} over the tolerance"
+        at += n
+
+
+def places(b, i, positions):
+    j = torch.as_tensor(positions, device="cuda")
+    return b.table[i].long()[j // b.page], j % b.page
+
+
+# (new tokens, page): the warps split the tokens; the warps split the rows; tensor memory
+KERNELS = [(1, 16), (40, 24), (40, 16), (130, 16)]
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("magnitude,ahead", [(-5, 10), (-10, 10), (-14, 7), (-14, 10), (-16, 0), (-20, 0), (-20, 10), (-30, 0), (-60, 3), (20, 5)])
+@pytest.mark.parametrize("zeros", ["one", "run", "last"])
+def test_value_heads_of_zeros_in_an_e4m3_cache(cuda, new, page, size, magnitude, ahead, zeros):
+    """A visible token whose value head is zero has the exponent byte 127, whatever the other values' magnitude 2^`magnitude`:
+    it takes its share of the weight and none of the others' bits.  Its score is about `ahead` above the others'."""
+    b = Batch(80, [300, 700], [new, new], 8, 2, size, page, torch.bfloat16, True)
+    b.q[..., 0] = 4
+    for i, n in enumerate(b.lengths):
+        page_, place = places(b, i, range(n))
+        b.kc.view(torch.uint8)[page_, place, :, 0] = 0
+        b.ve[page_, place] = (b.ve[page_, place].int() + magnitude).to(torch.uint8)
+        page_, place = places(b, i, {"one": [5], "run": range(0, 270), "last": [n - 20, n - 1]}[zeros])
+        b.kc.view(torch.uint8)[page_, place] = 0
+        b.kc[page_, place, :, 0] = torch.tensor(ahead * size ** 0.5 / 4, device="cuda").to(torch.float8_e4m3fn)
+        b.ke[page_, place] = 127
+        b.vc.view(torch.uint8)[page_, place] = 0
+        b.vc.view(torch.uint8)[page_, place, :, ::3] = 0x80            # -0
+        b.ve[page_, place] = 127
+    check(b, b.call())
+    if new == 1:
+        b.starts = None
+        check(b, b.call())
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+def test_one_key_head_has_no_values_at_all(cuda, new, page):
+    b = Batch(81, [300, 2100, 17], [new, new, 5], 8, 2, 128, page, torch.float16, True)
+    for i, n in enumerate(b.lengths):
+        page_, place = places(b, i, range(n))
+        b.vc.view(torch.uint8)[page_, place, 1] = 0
+        b.ve[page_, place, 1] = 127
+        b.ve[page_, place, 0] -= 9
+    out = b.call()
+    check(b, out)
+    assert bool((out[:, 4:] == 0).all())

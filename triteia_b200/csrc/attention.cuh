@@ -255,8 +255,9 @@ struct AttnCfg {
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
   // About 96 KB of loads in flight per CTA and two CTAs per SM: 6.5 TB/s for about 1.5 us of latency is 66 KB per SM.
   static constexpr int STAGES = 98304 / STAGE_BYTES > 6 ? 6 : 98304 / STAGE_BYTES;
-  static constexpr int MASK_OFF = STAGES * STAGE_BYTES;         // uint32 [STAGES][4]: tokens that count, per loading warp
-  static constexpr int EXP_OFF = MASK_OFF + STAGES * 16;        // float [STAGES][3][UNIT]: 2^e of keys; e and 2^-e of values
+  // uint32 [STAGES][4][2], per loading warp: tokens that count; e4m3: tokens that may have a value head of zeros
+  static constexpr int MASK_OFF = STAGES * STAGE_BYTES;
+  static constexpr int EXP_OFF = MASK_OFF + STAGES * 32;        // float [STAGES][3][UNIT]: 2^e of keys; e and 2^-e of values
   static constexpr int WML_OFF = EXP_OFF + (FP8 ? STAGES * 3 * UNIT * 4 : 0);   // float [4][16][2]: the warps' maxima and sums (M = 16)
   static constexpr int ML_OFF = WML_OFF + (ROWS ? 0 : 4 * 16 * 8);             // float [16][2]: the CTA's (M = 16)
   static constexpr int O_STRIDE = D + 4;                                       // floats
@@ -343,6 +344,37 @@ struct AttnMma<T, true> { using type = __half; };
 __device__ __forceinline__ int attn_row_shift(float top) {
   const int field = (int)(__float_as_uint(top) >> 23);                  // top in [2^(field - 127), twice that)
   return top > 0.f ? min(max(127 + 127 + 9 - field, 1), 253) : 127;
+}
+
+// A value head of zeros has the exponent byte 127 (kv_cache.cuh).  Its product with a weight is zero whatever exponent it is
+// given, but the running maximum below is over log2 weight + e: with e = 0 such a token would push the weights of values that
+// are all much smaller out of fp16.  It takes this exponent instead, below any that matters (values under 2^-81 alone are less),
+// while its weight times 2^90 enters the sum as ever: 2^(90 + 8) a token, far from the end of 32 bits for 2^17 tokens and more.
+constexpr int kZeroValueExp = -90;
+
+// Whether all of a head's `chunks` 16-byte pieces of codes are zeros, of either sign.
+template <int CHUNKS, class Load>
+__device__ __forceinline__ bool attn_zero_codes(Load load) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const uint4 w = load(c);
+    any |= w.x | w.y | w.z | w.w;
+  }
+  return (any & 0x7f7f7f7fu) == 0;
+}
+
+// Gives the tokens of `maybe` (byte 127) whose value codes in shared memory are zeros their exponent; a warp for itself.  Not
+// inlined: the loop that hardly ever calls it has to stay in the instruction cache.
+template <class Cfg>
+__device__ __noinline__ void attn_zero_values(unsigned long long maybe, uint32_t vbase, float* exps, int lane) {
+#pragma unroll 1
+  for (int r = lane; r < 16 * Cfg::NT; r += 32)
+    if ((maybe >> r) & 1 && attn_zero_codes<Cfg::CHUNKS>([&](int c) { return lds128(vbase + attn_swizzle<Cfg::ROWB>(r, c)); })) {
+      exps[Cfg::UNIT + r] = (float)kZeroValueExp;
+      exps[2 * Cfg::UNIT + r] = __uint_as_float((uint32_t)(127 - kZeroValueExp) << 23);
+    }
+  __syncwarp();
 }
 
 // Softmax state of a warp's 16 rows; a lane has rows lane / 4 and lane / 4 + 8.
@@ -572,7 +604,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
   const uint8_t* kc = static_cast<const uint8_t*>(a.key_cache);
   const uint8_t* vc = static_cast<const uint8_t*>(a.value_cache);
   constexpr int ESZ = Cfg::FP8 ? 1 : 2;
-  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Cfg::MASK_OFF);
+  uint2* masks = reinterpret_cast<uint2*>(smem + Cfg::MASK_OFF);
   float* exps = reinterpret_cast<float*>(smem + Cfg::EXP_OFF);
   constexpr int WTOK = Cfg::WTOK;                     // 16 or 32 tokens of a stage are this warp's to load
   const int tok = warp * WTOK + (lane & (WTOK - 1));  // this lane's among the unit's
@@ -587,9 +619,12 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     return {pg >= 0 && pg < a.num_pages ? pg : -1, j - p * a.page_size, ld.kvh};
   };
   Where ahead = where();
-  int exp_slot = -1, kb = 127, vb = 127;              // e4m3: the bytes that the last issue() asked for, and their stage
+  int exp_slot = -1, kb = 126, vb = 126;              // e4m3: the bytes that the last issue() asked for, and their stage
   auto settle_exps = [&]() {
-    if (exp_slot >= 0 && lane < WTOK) {
+    if (exp_slot < 0) return;
+    const unsigned maybe = __ballot_sync(0xffffffffu, vb == 127 && lane < WTOK);
+    if (lane == 0) masks[exp_slot * 4 + warp].y = maybe;
+    if (lane < WTOK) {
       float* e = exps + exp_slot * 3 * UNIT + tok;
       e[0] = pow2_of_byte(kb);
       e[UNIT] = (float)(vb - 127);
@@ -616,10 +651,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
       if constexpr (ESZ == 2) off *= 2;
       unsigned mask = __ballot_sync(0xffffffffu, there);
       if constexpr (WTOK == 16) mask &= 0xffffu;
-      if (lane == 0) masks[slot * 4 + warp] = mask;
+      if (lane == 0) masks[slot * 4 + warp].x = mask;
       if constexpr (Cfg::FP8) {
         exp_slot = slot;
-        kb = vb = 127;
+        kb = vb = 126;
         if (there) {
           const long long eo = (long long)w.page * a.e_page + (long long)w.place * a.e_tok + (long long)w.kvh * a.e_head;
           kb = a.key_exp[eo];
@@ -743,13 +778,24 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
         constexpr int TOK = Cfg::NT * 16;
         const int own = Cfg::ROWS ? 0 : warp * WTOK;
         const int j0 = u * UNIT + own;
-        const uint32_t* mk = masks + slot * 4;
-        const unsigned long long valid =
-            Cfg::ROWS ? (unsigned long long)(mk[0] | mk[1] << 16) | (unsigned long long)(mk[2] | mk[3] << 16) << 32 : mk[warp];
+        const uint2* mk = masks + slot * 4;
+        unsigned long long valid, maybe;
+        if constexpr (Cfg::ROWS) {
+          const uint2 m0 = mk[0], m1 = mk[1], m2 = mk[2], m3 = mk[3];
+          valid = (unsigned long long)(m0.x | m1.x << 16) | (unsigned long long)(m2.x | m3.x << 16) << 32;
+          maybe = (unsigned long long)(m0.y | m1.y << 16) | (unsigned long long)(m2.y | m3.y << 16) << 32;
+        } else {
+          const uint2 m = mk[warp];
+          valid = m.x;
+          maybe = m.y;
+        }
         constexpr unsigned long long kAll = ~0ull >> (64 - TOK);
         if (valid != 0) {
           const bool need_mask = valid != kAll || j0 + TOK > all_hi || j0 < all_lo;
           const uint32_t kbase = smem_base + slot * Cfg::STAGE_BYTES + own * Cfg::ROWB;
+          if constexpr (Cfg::FP8) {                   // the warps of the rows' form all mark all tokens, with the same values
+            if (maybe != 0) attn_zero_values<Cfg>(maybe, kbase + Cfg::HALF_BYTES, exps + slot * 3 * UNIT + own, lane);
+          }
           attn_block<T, Cfg, Cfg::NT>(st, q, c_row, kbase, kbase + Cfg::HALF_BYTES, exps + slot * 3 * UNIT + own, valid, j0, row_hi, row_lo,
                                       need_mask, lane);
         }

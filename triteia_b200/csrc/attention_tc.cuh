@@ -341,6 +341,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     // is waited for.
     const int first = (warp - 10) * 32 + lane;
     int page[2], place[2], kb[2], vb[2];              // of the next tile but one; of the next tile (-1: not there)
+    long long code_at[2];                             // the next tile's codes
     auto ask_pages = [&](int i) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -358,10 +359,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         kb[x] = vb[x] = -1;
+        code_at[x] = 0;
         if (page[x] >= 0 && page[x] < a.num_pages) {
           const long long at = (long long)page[x] * a.e_page + (long long)place[x] * a.e_tok + (long long)kvh * a.e_head;
           kb[x] = a.key_exp[at];
           vb[x] = a.value_exp[at];
+          code_at[x] = (long long)page[x] * a.c_page + (long long)place[x] * a.c_tok + (long long)kvh * a.c_head;
         }
       }
     };
@@ -373,12 +376,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       const int s = i & 1;
       // The slot is free once the converting warps have its factors and every softmax that uses the tile its exponents.
       mbar_wait(&fac_free[s], ((i >> 1) & 1) ^ 1, dead);
+      // A value head of zeros (byte 127) takes the tile's exponent, whatever it is, and has no part in it.
+      if (__any_sync(0xffffffffu, vb[0] == 127 || vb[1] == 127)) {
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          const uint4* codes = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.value_cache) + code_at[x]);
+          if (vb[x] == 127 && attn_zero_codes<D / 16>([&](int c) { return codes[c]; })) vb[x] = -1;
+        }
+      }
       const int2 most = make_int2(__reduce_max_sync(0xffffffffu, max(kb[0], kb[1])), __reduce_max_sync(0xffffffffu, max(vb[0], vb[1])));
       if (lane == 0) maxima[2 * s + (warp - 10)] = most;
       named_bar_sync(1, 64);
       const int2 m0 = maxima[2 * s], m1 = maxima[2 * s + 1];
       int ek = max(m0.x, m1.x), ev = max(m0.y, m1.y);
-      if (ek < 0) ek = ev = 127;                      // no token of the tile is there
+      if (ek < 0) ek = 127;                           // no token of the tile is there
+      if (ev < 0) ev = 127 + kZeroValueExp;           // nor one whose values are not all zeros
       float* e = reinterpret_cast<float*>(smem + Cfg::EXP_OFF) + s * Cfg::EXP_FLOATS;
       __half* scales = reinterpret_cast<__half*>(smem + Cfg::SCALE_OFF) + s * 256;
       bool any = false;

@@ -1,5 +1,6 @@
 """A paged cache of keys and values: [pages, page_size, kv_heads, head_size], in the model's type or as e4m3 codes with one
-exponent byte b per token and head (value = code * 2^(b - 127)).  A token's slot is page * page_size + place."""
+exponent byte b per token and head (value = code * 2^(b - 127); 127 for a head of zeros, also in a cache that is filled by other
+means: paged_attention knows such heads by it).  A token's slot is page * page_size + place."""
 import torch
 
 from ..._lib import load_binding
