@@ -71,3 +71,27 @@ def test_one_key_head_has_no_values_at_all(cuda, new, page):
     out = b.call()
     check(b, out)
     assert bool((out[:, 4:] == 0).all())
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("small", [-20, -40])
+def test_tiny_values_with_all_the_weight(cuda, new, page, size, small):
+    """Every third token has values 2^`small` times the others' and all of the weight (the others' scores are hundreds below),
+    so that only the tiny ones' magnitude may enter the tolerance."""
+    b = Batch(82, [300, 170], [new, new], 8, 2, size, page, torch.bfloat16, True)
+    vmax = 0.0
+    for i, n in enumerate(b.lengths):
+        page_, place = places(b, i, range(n))
+        tiny = torch.arange(n, device="cuda") % 3 == 0
+        e = b.ve[page_, place].int()
+        b.ve[page_, place] = torch.where(tiny[:, None], e + small, e).to(torch.uint8)
+        keys = b.kc[page_, place].float()
+        keys = torch.where(tiny[:, None, None], keys, torch.full_like(keys, -448.0))
+        b.kc.view(torch.uint8)[page_, place] = keys.to(torch.float8_e4m3fn).view(torch.uint8)
+        vmax = max(vmax, float(b.tokens(i)[1][tiny].abs().max()))
+    b.q = b.q.abs() + 0.25
+    out = b.call()
+    check(b, out, vmax=vmax)
+    with pytest.raises(AssertionError):
+        check(b, torch.zeros_like(out), vmax=vmax)
