@@ -95,3 +95,48 @@ def test_tiny_values_with_all_the_weight(cuda, new, page, size, small):
     check(b, out, vmax=vmax)
     with pytest.raises(AssertionError):
         check(b, torch.zeros_like(out), vmax=vmax)
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("larger", [12, 17, 24, 30, 100])
+@pytest.mark.parametrize("where", ["hidden", "orthogonal"])
+def test_a_key_that_dwarfs_its_neighbours(cuda, new, page, size, larger, where):
+    """One key 2^`larger` times its neighbours' takes no bits of their scores: rows that do not see it, or are orthogonal to it."""
+    b = Batch(83, [300, 2100], [new, new], 8, 2, size, page, torch.bfloat16, True)
+    for i, n in enumerate(b.lengths):
+        if where == "hidden":
+            page_, place = places(b, i, [n - 1])
+        else:
+            page_, place = places(b, i, [n - 30, 3])
+            b.kc.view(torch.uint8)[page_, place, :, 1:] = 0
+            b.kc[page_, place, :, 0] = torch.tensor(300.0, device="cuda").to(torch.float8_e4m3fn)
+        b.ke[page_, place] += larger
+    if where == "orthogonal":
+        b.q[..., 0] = 0
+    out = b.call()
+    if where == "hidden":                      # the last row of each sequence sees the large key: its scores may be anything
+        b.new = [new - 1, new - 1]
+        keep = torch.ones(2 * new, dtype=torch.bool, device="cuda")
+        keep[[new - 1, 2 * new - 1]] = False
+        b.q, out = b.q[keep], out[keep]
+        for i in range(2):
+            b.lengths[i] -= 1
+        if new == 1:
+            return
+    check(b, out)
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+@pytest.mark.parametrize("small", [-16, -24, -60])
+def test_key_heads_of_zeros_among_small_keys(cuda, new, page, small):
+    """A key head of zeros has the exponent byte 127 and a score of zero; the other keys, 2^`small`, keep their bits."""
+    b = Batch(84, [300, 700], [new, new], 8, 2, 128, page, torch.bfloat16, True)
+    for i, n in enumerate(b.lengths):
+        page_, place = places(b, i, range(n))
+        b.ke[page_, place] = (b.ke[page_, place].int() + small).to(torch.uint8)
+        page_, place = places(b, i, range(7, n, 50))
+        b.kc.view(torch.uint8)[page_, place] = 0
+        b.ke[page_, place] = 127
+    scale = 128 ** -0.5 * 2.0 ** -small
+    check(b, b.call(scale=scale), scale=scale)

@@ -53,8 +53,9 @@ struct AttnTcCfg {
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int CODE_OFF = KV_OFF + BUFS * TILE_BYTES;
-  // e4m3, per key tile modulo 2: 2^E of the keys, E of the values, 2^-E, whether values have rests, the rests [128].
-  static constexpr int EXP_OFF = CODE_OFF + CODE_BUFS * CODE_BYTES, EXP_FLOATS = 4 + 128;
+  // e4m3, per key tile modulo 2: 2^E of the keys, E of the values, 2^-E, whether keys or values have rests; the values' rests
+  // [128]; the powers that the keys' scores still need [128].
+  static constexpr int EXP_OFF = CODE_OFF + CODE_BUFS * CODE_BYTES, EXP_FLOATS = 4 + 2 * 128;
   static constexpr int SCALE_OFF = EXP_OFF + (FP8 ? 2 * EXP_FLOATS * 4 : 0);      // fp16 [2][2][128]: factors of keys and values
   static constexpr int MAX_OFF = SCALE_OFF + (FP8 ? 2 * 2 * 128 * 2 : 0);         // int [2][2][2]: two warps' largest exponents
   static constexpr int BAR_OFF = MAX_OFF + (FP8 ? 32 : 0);
@@ -135,6 +136,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// Whether the codes of a head that begins `at` bytes into a cache are zeros.  Not inlined: hardly ever called.
+template <int CHUNKS>
+__device__ __noinline__ bool attn_tc_zero_head(const void* cache, long long at) {
+  const uint4* codes = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + at);
+  return attn_zero_codes<CHUNKS>([&](int c) { return codes[c]; });
 }
 
 // SPLIT: the 2, 4 or 8 CTAs of a cluster share an item, each with a run of its key tiles.  At the end CTA r finishes the rows of
@@ -376,12 +384,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       const int s = i & 1;
       // The slot is free once the converting warps have its factors and every softmax that uses the tile its exponents.
       mbar_wait(&fac_free[s], ((i >> 1) & 1) ^ 1, dead);
-      // A value head of zeros (byte 127) takes the tile's exponent, whatever it is, and has no part in it.
-      if (__any_sync(0xffffffffu, vb[0] == 127 || vb[1] == 127)) {
-#pragma unroll 1
+      // A head of zeros (byte 127) takes the tile's exponent, whatever it is, and has no part in it.
+      if (__any_sync(0xffffffffu, kb[0] == 127 || kb[1] == 127 || vb[0] == 127 || vb[1] == 127)) {
+#pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint4* codes = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.value_cache) + code_at[x]);
-          if (vb[x] == 127 && attn_zero_codes<D / 16>([&](int c) { return codes[c]; })) vb[x] = -1;
+          if (kb[x] == 127 && attn_tc_zero_head<D / 16>(a.key_cache, code_at[x])) kb[x] = -1;
+          if (vb[x] == 127 && attn_tc_zero_head<D / 16>(a.value_cache, code_at[x])) vb[x] = -1;
         }
       }
       const int2 most = make_int2(__reduce_max_sync(0xffffffffu, max(kb[0], kb[1])), __reduce_max_sync(0xffffffffu, max(vb[0], vb[1])));
@@ -389,20 +397,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       named_bar_sync(1, 64);
       const int2 m0 = maxima[2 * s], m1 = maxima[2 * s + 1];
       int ek = max(m0.x, m1.x), ev = max(m0.y, m1.y);
-      if (ek < 0) ek = 127;                           // no token of the tile is there
-      if (ev < 0) ev = 127 + kZeroValueExp;           // nor one whose values are not all zeros
+      if (ek < 0) ek = 127;                           // no token of the tile is there, or all of its keys are zeros
+      if (ev < 0) ev = 127 + kZeroValueExp;           // the same of its values
       float* e = reinterpret_cast<float*>(smem + Cfg::EXP_OFF) + s * Cfg::EXP_FLOATS;
       __half* scales = reinterpret_cast<__half*>(smem + Cfg::SCALE_OFF) + s * 256;
       bool any = false;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int tok = first + 64 * x;
-        const int kd = ek - kb[x], vd = min(ev - vb[x], 15);
+        const int kd = min(ek - kb[x], 15), vd = min(ev - vb[x], 15);
         const float rest = vb[x] >= 0 ? (float)(vb[x] + vd - ev) : 0.f;
-        scales[tok] = kd > 24 ? __float2half_rn(0.f) : __float2half_rn(pow2_of_byte(127 - kd));
+        const int k_up = kb[x] >= 0 ? kb[x] + kd : ek;
+        scales[tok] = __float2half_rn(pow2_of_byte(127 - kd));
         scales[128 + tok] = __float2half_rn(pow2_of_byte(127 - vd));
         e[4 + tok] = rest;
-        any |= rest != 0.f;
+        e[132 + tok] = pow2_of_byte(k_up);
+        any |= rest != 0.f || k_up != ek;
       }
       any = __any_sync(0xffffffffu, any);
       if (lane == 0) reinterpret_cast<uint16_t*>(e + 3)[warp - 10] = any ? 1 : 0;      // two halves, read as one number
@@ -568,8 +578,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       const int j0 = (kt0 + i) * 128;
       mbar_wait(&s_bar[tile], i & 1, dead);
       tc_fence_after();
-      // e4m3: the tile's codes carry 2^(e_j - E) already, E the largest exponent of the tile (one for keys, one for values);
-      // values further than 2^15 below the largest of their tile would leave fp16 and keep a rest, which enters per token.
+      // e4m3: the tile's codes carry 2^(e_j - E) already, E the largest exponent of the tile (one for keys, one for values).
+      // Further than 2^15 below, codes would lose bits in fp16: they carry 2^-15 and the token keeps a rest, values in the
+      // exponent of the weight, keys in the factor of the score.
       float ct = c, add = 0.f, back = 1.f;
       const float* fac = nullptr;
       bool rests = false;
@@ -604,7 +615,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           tc_wait_ld32(w);
           if (rests) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) w[x] = __float_as_uint(fmaf(__uint_as_float(w[x]), ct, fac[4 + b * 32 + x]));
+            for (int x = 0; x < 32; x += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(fac + 132 + b * 32 + x), r4 = *reinterpret_cast<const float4*>(fac + 4 + b * 32 + x);
+              w[x] = __float_as_uint(fmaf(__uint_as_float(w[x]), c * k4.x, r4.x));
+              w[x + 1] = __float_as_uint(fmaf(__uint_as_float(w[x + 1]), c * k4.y, r4.y));
+              w[x + 2] = __float_as_uint(fmaf(__uint_as_float(w[x + 2]), c * k4.z, r4.z));
+              w[x + 3] = __float_as_uint(fmaf(__uint_as_float(w[x + 3]), c * k4.w, r4.w));
+            }
           }
           mask(w, seen(b));
           tc_st32(s_addr + b * 32, w);
@@ -663,7 +680,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       const float off = kBias + add - (m == -INFINITY ? 0.f : m);
       const float2 c2 = make_float2(cs, cs), off2 = make_float2(off, off);
       float2 sum = make_float2(0.f, 0.f);
-      float rest_sum = 0.f;                           // of the weights without the values' rests
+      float rest_sum = 0.f;                           // of the weights without the values' exponents
       if (Cfg::FP8 && rests) {
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
@@ -671,7 +688,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           tc_ld32(s_addr + b * 32, w);
           tc_wait_ld32(w);
 #pragma unroll
-          for (int x = 0; x < 32; ++x) rest_sum += exp2_fast(__uint_as_float(w[x]) + off - fac[4 + b * 32 + x]);
+          for (int x = 0; x < 32; x += 4) {
+            const float4 r4 = *reinterpret_cast<const float4*>(fac + 4 + b * 32 + x);
+            rest_sum += exp2_fast(__uint_as_float(w[x]) - r4.x + (off - add));
+            rest_sum += exp2_fast(__uint_as_float(w[x + 1]) - r4.y + (off - add));
+            rest_sum += exp2_fast(__uint_as_float(w[x + 2]) - r4.z + (off - add));
+            rest_sum += exp2_fast(__uint_as_float(w[x + 3]) - r4.w + (off - add));
+          }
         }
       }
 #pragma unroll
@@ -699,7 +722,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
           if (lane == 0) mbar_arrive(&p_bar[2 * tile + (b >> 1)]);
         }
       }
-      l = fmaf(rests ? rest_sum : sum.x + sum.y, back, l);
+      l = rests ? l + rest_sum : fmaf(sum.x + sum.y, back, l);
       if (Cfg::FP8 && lane == 0) mbar_arrive(&fac_free[i & 1]);
     }
     if (Cfg::FP8) {                                   // the other tile's last key tiles: this one has no use for them
