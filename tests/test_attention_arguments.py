@@ -189,3 +189,8 @@ def test_a_missing_binding_fails_loudly(monkeypatch):
     monkeypatch.delattr(triteia_b200, "_binding", raising=False)
     with pytest.raises(ImportError, match="no CPU"):
         _lib.load_binding()
+
+
+def test_a_window_that_leaves_32_bits_is_refused():
+    """Positions run from -num_tokens to the table's width, and a window is subtracted from them."""
+    assert _attention(table_width=1 << 25, page_size=63, num_tokens=1 << 29, window=5) == 1

@@ -140,3 +140,15 @@ def test_key_heads_of_zeros_among_small_keys(cuda, new, page, small):
         b.ke[page_, place] = 127
     scale = 128 ** -0.5 * 2.0 ** -small
     check(b, b.call(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(torch.float16, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 40, 2 ** 31 - 300, 1 << 20])
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("plan", [SHORT, LONG_SHORT, ([3], [7]), ([5, 300], [1, 1])], ids=["short", "long-short", "one", "single"])
+def test_windows_that_hide_nothing(cuda, dtype, e4m3, window, page, plan):
+    """Any window as long as the sequences or longer, also with more new tokens than the cache has."""
+    b = Batch(85, *plan, 8, 2, 128, page, dtype, e4m3)
+    out = b.call(window=window)
+    b.check(out)
+    assert torch.equal(out, b.call())

@@ -85,8 +85,12 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
   if ((query_token_stride | query_head_stride | out_token_stride | out_head_stride) & 7) return TRB_ERR_PROB_SHAPE;
   if (((page_stride | token_stride | head_stride) * esz) & 15) return TRB_ERR_PROB_SHAPE;
   // Positions are 32-bit numbers; the largest unit starts below length + 64.
-  if ((long long)table_width * page_size > 0x7fff0000LL || (long long)num_tokens * (num_heads / num_kv_heads) > 0x7fff0000LL)
-    return TRB_ERR_PROB_SHAPE;
+  const long long most = (long long)table_width * page_size;
+  if (most > 0x7fff0000LL || (long long)num_tokens * (num_heads / num_kv_heads) > 0x7fff0000LL) return TRB_ERR_PROB_SHAPE;
+  // A window as wide as the table hides nothing.  A narrower one is subtracted from positions down to -num_tokens (more new tokens
+  // than the cache has).
+  if (window >= most) window = 0;
+  if (window > 0 && most + num_tokens > 0x7fff0000LL) return TRB_ERR_PROB_SHAPE;
   if (dtype != TRB_F16 && dtype != TRB_BF16) return TRB_ERR_KERN_SHAPE;
   if (head_size != 64 && head_size != 128) return TRB_ERR_KERN_SHAPE;
   DeviceGuard guard(dev);
