@@ -283,6 +283,17 @@ int trb_paged_attention(const void* query, const void* key_cache, const void* va
                         long long out_head_stride, long long page_stride, long long token_stride, long long head_stride,
                         long long exp_page_stride, long long exp_token_stride, long long exp_head_stride, float scale,
                         int causal, int window, int dtype, void* workspace, size_t workspace_bytes, int dev, void* stream);
+/* The same; clear != 0 (query_starts given): rows of out outside every sequence become zero. */
+int trb_paged_attention_clear(const void* query, const void* key_cache, const void* value_cache,
+                              const void* key_exponents, const void* value_exponents, const void* page_table,
+                              const void* lengths, const void* query_starts, void* out, int num_tokens, int num_seqs,
+                              int num_heads, int num_kv_heads, int head_size, int page_size, long long num_pages,
+                              long long table_stride, int table_width, long long query_token_stride,
+                              long long query_head_stride, long long out_token_stride, long long out_head_stride,
+                              long long page_stride, long long token_stride, long long head_stride,
+                              long long exp_page_stride, long long exp_token_stride, long long exp_head_stride,
+                              float scale, int causal, int window, int dtype, void* workspace, size_t workspace_bytes,
+                              int dev, void* stream, int clear);
 /* Working memory of that call (16-byte aligned, no initial contents needed, free again when the call has finished on the
  * device): pieces of the sequences that more than one CTA reads.  single: query_starts is NULL; e4m3: there are exponents. */
 size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,

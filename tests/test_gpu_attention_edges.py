@@ -152,3 +152,77 @@ def test_windows_that_hide_nothing(cuda, dtype, e4m3, window, page, plan):
     out = b.call(window=window)
     b.check(out)
     assert torch.equal(out, b.call())
+
+
+def spoiled(shape, dtype):
+    """Leaves a block of NaN of this size to the allocator."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    x = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+    torch.cuda.synchronize()
+    del x
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,new,front,behind", [
+    ([300, 170], [40, 130], 0, 70), ([300, 170], [40, 130], 9, 3), ([0, 0], [0, 0], 0, 50), ([40, 70], [2, 1], 0, 29), ([4000, 70], [2, 1], 2, 29),
+    ([5000], [1], 0, 1), ([100], [1], 3, 500), ([4000, 9], [64, 3], 5, 700), ([300, 170], [40, 130], 0, 0)])
+@pytest.mark.parametrize("page", [16, 24])
+def test_rows_of_no_sequence_are_zero_in_a_new_output(cuda, e4m3, lengths, new, front, behind, page):
+    b = Batch(86, lengths, new, 8, 2, 128, page, torch.float16, e4m3)
+    T = sum(new)
+    q = torch.full((front + T + behind, 8, 128), float("nan"), dtype=torch.float16, device="cuda")
+    q[front:front + T] = b.q
+    b.q, b.starts = q, b.starts + front
+    spoiled(q.shape, q.dtype)
+    out = b.call()
+    assert bool((out[:front] == 0).all()) and bool((out[front + T:] == 0).all())
+    given = torch.full_like(q, 3)
+    b.call(out=given)
+    assert bool((given[:front] == 3).all()) and bool((given[front + T:] == 3).all()) and torch.equal(given[front:front + T], out[front:front + T])
+    b.q = q[front:front + T]
+    b.check(out[front:front + T])
+
+
+def test_a_batch_without_sequences_is_all_padding(cuda):
+    kc, vc, _, _ = ops.new_cache(2, 16, 2, 64)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    q = torch.full((5000, 4, 64), float("nan"), dtype=torch.float16, device="cuda")
+    spoiled(q.shape, q.dtype)
+    for width in (0, 3):
+        out = ops.paged_attention(q, kc, vc, none.new_zeros(0, width), none, none.new_zeros(1))
+        assert bool((out == 0).all())
+    given = torch.full_like(q, 3)
+    ops.paged_attention(q, kc, vc, none.new_zeros(0, 3), none, none.new_zeros(1), out=given)
+    assert bool((given == 3).all())
+
+
+def test_delta_attention_of_a_padded_batch(cuda):
+    """Padding tokens behind the last sequence (slot -1, position -1): the live rows are those of the batch without them, and the
+    output projection gets zeros for the others."""
+    from triteia_b200.nn import delta_attention
+
+    hidden, heads, kv_heads, size, page = 512, 4, 2, 128, 16
+    m = delta_attention(hidden, heads, kv_heads, size, 2, max_position=128, groupsize=128).to(cuda)
+    g = gen(87)
+    for name, k, n in (("qkv", hidden, 8 * size), ("o", heads * size, hidden)):
+        q, meta, s = ops.random_packed_deltas(2, k, n, groupsize=128, device=cuda, seed=1, scale_lo=0.002, scale_hi=0.004)
+        getattr(m, name + "_qweight").copy_(q), getattr(m, name + "_meta").copy_(meta), getattr(m, name + "_scale").copy_(s)
+        getattr(m, name + "_weight").copy_(normal(g, n, k) * k ** -0.5)
+    angle = torch.outer(torch.arange(128, device="cuda").double(), 10000.0 ** (-torch.arange(0, size, 2, device="cuda").double() / size))
+    m.cos_sin_cache.copy_(torch.cat([angle.cos(), angle.sin()], 1))
+    table = torch.tensor([[4, 1, -1], [0, 3, 5]], dtype=torch.int32, device="cuda")
+    new, T, pad = [20, 33], 53, 11
+    x = normal(g, T + pad, hidden)
+    pos = torch.cat([torch.arange(n, device="cuda") for n in new] + [torch.full((pad,), -1, device="cuda")])
+    seq = torch.cat([torch.full((n,), i, device="cuda") for i, n in enumerate(new)])
+    slots = torch.cat([table[seq, pos[:T] // page].long() * page + pos[:T] % page, torch.full((pad,), -1, device="cuda")])
+    idx = torch.cat([torch.tensor([1, -1], dtype=torch.int32, device="cuda")[seq], torch.full((pad,), -1, dtype=torch.int32, device="cuda")])
+    lengths, starts = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (new, [0, 20, 53]))
+    outs = []
+    for rows in (T + pad, T):
+        cache = ops.new_cache(6, page, kv_heads, size, torch.float16, False)
+        spoiled((rows, heads, size), torch.float16)
+        outs.append(m(x[:rows], idx[:rows], pos[:rows], slots[:rows], cache, table, lengths, starts))
+    assert torch.equal(outs[0][:T], outs[1])
+    assert bool((outs[0][T:] == 0).all())

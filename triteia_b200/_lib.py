@@ -48,6 +48,7 @@ SIGNATURES = {
     "trb_cache_write": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 11 + [_i, _i, _vp]),
     "trb_cache_read": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 7 + [_i, _i, _vp]),
     "trb_paged_attention": (_i, [_vp] * 9 + [_i] * 6 + [_ll, _ll, _i] + [_ll] * 10 + [_f] + [_i] * 3 + [_vp, _sz, _i, _vp]),
+    "trb_paged_attention_clear": (_i, [_vp] * 9 + [_i] * 6 + [_ll, _ll, _i] + [_ll] * 10 + [_f] + [_i] * 3 + [_vp, _sz, _i, _vp, _i]),
     "trb_paged_attention_workspace_bytes": (_sz, [_i] * 10),
     "trb_row_checksum": (_i, [_vp] * 2 + [_i] * 4 + [_vp]),
     "trb_stack_scratch_bytes": (_sz, [_i, _i]),

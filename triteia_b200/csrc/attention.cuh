@@ -45,6 +45,7 @@ struct AttnArgs {
   int tokens, seqs, kv_heads, group, page_size, table_width;
   int page_shift;                     // log2(page_size), -1 where that is no integer
   int causal, window;
+  int clear;                          // rows of out that belong to no sequence become zero
 };
 
 // One work tile: rows [row0, row0 + M) of sequence `seq`, whose new tokens are rows of the query from `q0`.
@@ -67,6 +68,24 @@ __device__ __forceinline__ void attn_query_range(const AttnArgs& a, int b, int& 
 __device__ __forceinline__ int attn_length(const AttnArgs& a, int b) {
   const long long most = (long long)a.table_width * a.page_size;
   return (int)max(0LL, min((long long)a.lengths[b], most));
+}
+
+// This CTA's share of the rows of out before the first and behind the last sequence; `thread` of `threads` take part.
+template <class T, int D>
+__device__ __forceinline__ void attn_clear_rest(const AttnArgs& a, int thread, int threads) {
+  const int first = max(0, min(a.query_starts[0], a.tokens)), last = max(first, min(a.query_starts[a.seqs], a.tokens));
+  const int rest = first + (a.tokens - last), pieces = a.kv_heads * a.group * (D / 8);      // pieces of 16 bytes
+  for (int x = blockIdx.x; x < rest; x += gridDim.x) {
+    T* row = static_cast<T*>(a.out) + (long long)(x < first ? x : last + (x - first)) * a.o_tok;
+    for (int i = thread; i < pieces; i += threads)
+      *reinterpret_cast<uint4*>(row + (long long)(i / (D / 8)) * a.o_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// The same by itself, for a call without sequences.
+template <class T, int D>
+__global__ void __launch_bounds__(128) attn_clear_kernel(const AttnArgs a) {
+  attn_clear_rest<T, D>(a, threadIdx.x, 128);
 }
 
 // The `index`-th tile of the batch; all lanes of a warp call it together.  False: there are fewer tiles.
@@ -580,6 +599,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     f0 = skip;
     f1 = (uint32_t)it.n * (part + 1) / parts;
   } else if (pieces == nullptr) {       // a CTA for each item
+    if (a.clear) attn_clear_rest<T, D>(a, tid, Cfg::THREADS);
     if (!attn_find_tile<M>(a, blockIdx.x / a.kv_heads, it.t)) return;
     it.kvh = blockIdx.x % a.kv_heads;
     attn_item_units<M, UNIT>(a, it);
@@ -588,6 +608,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) attn_kernel(const AttnArgs a,
     f1 = it.n;
   } else {
     pdl_launch_dependents();            // the joining launch waits for this one's end before it reads
+    if (a.clear && gridDim.x == 1) attn_clear_rest<T, D>(a, tid, Cfg::THREADS);      // else the joining launch does
     long long own;
     const long long total = attn_total_units<M, UNIT>(a, own);
     const AttnRuns runs(total, gridDim.x);
@@ -989,6 +1010,7 @@ template <class T, class Cfg>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs a, const float* pieces, int ctas) {
   constexpr int D = Cfg::D, M = Cfg::M, UNIT = Cfg::UNIT;
   __shared__ float states[kJoinWarps][10][32];
+  if (a.clear && blockIdx.y == 0) attn_clear_rest<T, D>(a, threadIdx.x, kJoinWarps * 32);
   long long own;
   const long long total = attn_total_units<M, UNIT>(a, own);
   const int c = blockIdx.x;

@@ -32,6 +32,12 @@ static auto attn_with_cfg(bool fp8, int head_size, bool rows, F f) {
 template <class T>
 static int launch_attn(const AttnArgs& a, int head_size, void* workspace, size_t workspace_bytes, int dev, cudaStream_t st) {
   const bool fp8 = a.key_exp != nullptr;
+  if (a.seqs == 0) {
+    const unsigned ctas = a.tokens < 4096 ? a.tokens : 4096;
+    if (head_size == 128) attn_clear_kernel<T, 128><<<ctas, 128, 0, st>>>(a);
+    else attn_clear_kernel<T, 64><<<ctas, 128, 0, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
+  }
   const AttnKind kind = attn_kind(a.tokens, a.seqs, a.group, a.query_starts == nullptr, attn_tc_fits(a));
   if (kind == kAttnTensor) {
     if (head_size == 128) return fp8 ? launch_attn_tc<T, 128, true>(a, dev, st) : launch_attn_tc<T, 128, false>(a, dev, st);
@@ -58,21 +64,23 @@ extern "C" size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_se
   });
 }
 
-extern "C" int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
-                                   const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,
-                                   void* out, int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size, int page_size,
-                                   long long num_pages, long long table_stride, int table_width, long long query_token_stride,
-                                   long long query_head_stride, long long out_token_stride, long long out_head_stride,
-                                   long long page_stride, long long token_stride, long long head_stride, long long exp_page_stride,
-                                   long long exp_token_stride, long long exp_head_stride, float scale, int causal, int window, int dtype,
-                                   void* workspace, size_t workspace_bytes, int dev, void* stream) {
+extern "C" int trb_paged_attention_clear(const void* query, const void* key_cache, const void* value_cache,
+                                         const void* key_exponents, const void* value_exponents, const void* page_table,
+                                         const void* lengths, const void* query_starts, void* out, int num_tokens, int num_seqs,
+                                         int num_heads, int num_kv_heads, int head_size, int page_size, long long num_pages,
+                                         long long table_stride, int table_width, long long query_token_stride,
+                                         long long query_head_stride, long long out_token_stride, long long out_head_stride,
+                                         long long page_stride, long long token_stride, long long head_stride,
+                                         long long exp_page_stride, long long exp_token_stride, long long exp_head_stride,
+                                         float scale, int causal, int window, int dtype, void* workspace, size_t workspace_bytes,
+                                         int dev, void* stream, int clear) {
   using namespace trb;
-  if (num_tokens == 0 || num_seqs == 0) return TRB_OK;
+  if (num_tokens == 0 || (num_seqs == 0 && !clear)) return TRB_OK;
   const bool fp8 = key_exponents != nullptr;
-  if (num_tokens < 0 || num_seqs < 0 || !query || !key_cache || !value_cache || !lengths || !out || fp8 != (value_exponents != nullptr) ||
-      num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0) || window < 0)
+  if (num_tokens < 0 || num_seqs < 0 || !query || !key_cache || !value_cache || (!lengths && num_seqs > 0) || !out || fp8 != (value_exponents != nullptr) ||
+      num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0 && num_seqs > 0) || window < 0)
     return TRB_ERR_BAD_ARG;
-  if (!query_starts && num_tokens != num_seqs) return TRB_ERR_BAD_ARG;
+  if (!query_starts && (num_tokens != num_seqs || clear)) return TRB_ERR_BAD_ARG;
   // The stride of a dimension of one entry says nothing.
   if (num_kv_heads == 1) head_stride = head_size;
   if (page_size == 1) token_stride = head_size;
@@ -100,7 +108,23 @@ extern "C" int trb_paged_attention(const void* query, const void* key_cache, con
                    out_token_stride, out_head_stride, page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride,
                    exp_head_stride, table_stride, num_pages, scale * 1.4426950408889634f, num_tokens, num_seqs, num_kv_heads,
                    num_heads / num_kv_heads, page_size, table_width,
-                   (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1, causal, window};
+                   (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1, causal, window, clear != 0};
   if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, workspace, workspace_bytes, dev, (cudaStream_t)stream);
   return launch_attn<__nv_bfloat16>(a, head_size, workspace, workspace_bytes, dev, (cudaStream_t)stream);
+}
+
+extern "C" int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
+                                   const void* value_exponents, const void* page_table, const void* lengths,
+                                   const void* query_starts, void* out, int num_tokens, int num_seqs, int num_heads,
+                                   int num_kv_heads, int head_size, int page_size, long long num_pages, long long table_stride,
+                                   int table_width, long long query_token_stride, long long query_head_stride,
+                                   long long out_token_stride, long long out_head_stride, long long page_stride,
+                                   long long token_stride, long long head_stride, long long exp_page_stride,
+                                   long long exp_token_stride, long long exp_head_stride, float scale, int causal, int window,
+                                   int dtype, void* workspace, size_t workspace_bytes, int dev, void* stream) {
+  return trb_paged_attention_clear(query, key_cache, value_cache, key_exponents, value_exponents, page_table, lengths, query_starts,
+                                   out, num_tokens, num_seqs, num_heads, num_kv_heads, head_size, page_size, num_pages,
+                                   table_stride, table_width, query_token_stride, query_head_stride, out_token_stride,
+                                   out_head_stride, page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride,
+                                   exp_head_stride, scale, causal, window, dtype, workspace, workspace_bytes, dev, stream, 0);
 }

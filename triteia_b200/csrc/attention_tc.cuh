@@ -175,7 +175,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   const int item = SPLIT ? blockIdx.x / split : blockIdx.x, rank = SPLIT ? blockIdx.x % split : 0;
   const int kvh = item % a.kv_heads;
   AttnTile t;
-  if (!attn_find_tile<256>(a, tiles_bound - 1 - item / a.kv_heads, t)) return;
+  if (!attn_find_tile<256>(a, tiles_bound - 1 - item / a.kv_heads, t)) {
+    if (a.clear) attn_clear_rest<T, D>(a, tid, Cfg::THREADS);
+    return;
+  }
   int lo, hi;
   attn_key_range(a, t, lo, hi);
   // Key tiles [kt0, kt0 + n[i]) of this CTA concern the rows of tile i.
@@ -430,6 +433,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       ask_pages(i + 2);
     }
    }
+   if (warp >= 10 && a.clear) attn_clear_rest<T, D>(a, tid - 320, 64);      // these warps have the least to do
    if constexpr (SPLIT) {
      __syncwarp();
      cluster_sync_all();

@@ -238,12 +238,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::Tensor workspace;
   const size_t bytes = trb_paged_attention_workspace_bytes(T, B, heads, c.heads, size, c.page_size, width, starts == nullptr, c.key_exp != nullptr, dev);
   if (bytes > 0) workspace = fresh_tensor({(int64_t)bytes}, at::kByte, device);
-  const int status = trb_paged_attention(
+  // Rows of a new tensor that belong to no sequence are zeros, not what lay in the memory before.
+  const int status = trb_paged_attention_clear(
       ptr(query), ptr(c.key), ptr(c.value), ptr(c.key_exp), ptr(c.value_exp), ptr(table), ptr(lengths), ptr(starts), out_ptr(*out), T, B,
       heads, c.heads, size, c.page_size, c.pages, table.stride(0), width, query.stride(0),
       query.stride(1), out->stride(0), out->stride(1), c.page, c.token, c.head, c.e_page, c.e_token, c.e_head, (float)scale, causal,
       (int)(window > 0x7fffffff ? 0x7fffffff : window), tag,
-      bytes > 0 ? out_ptr(workspace) : nullptr, bytes, dev, stream_of(dev));
+      bytes > 0 ? out_ptr(workspace) : nullptr, bytes, dev, stream_of(dev), fresh.defined() && starts);
   check_status(status, "paged_attention", "heads of 64 or 128 that begin on 16-byte boundaries are needed");
   if (!fresh.defined()) return Py_NewRef(args[11]);
   return THPVariable_Wrap(std::move(fresh));

@@ -35,7 +35,8 @@ class delta_attention(nn.Module):
     def forward(self, x, indices, positions, slots, cache, page_table, lengths, query_starts=None):
         """x [T, hidden] fp16, the new tokens of the batch's sequences one after the other; indices [T] delta ids (-1: base model);
         positions int64 [T]; slots int64 [T], where their keys and values go; cache: what new_cache returned; page_table,
-        lengths (the new tokens included) and query_starts as paged_attention takes them."""
+        lengths (the new tokens included) and query_starts as paged_attention takes them.  Rows of x behind the last sequence are
+        padding (slot -1, position -1): their rows of the output projection's input are zero."""
         q_end = self.heads * self.head_size
         k_end = q_end + self.kv_heads * self.head_size
         qkv = sbmm_4bit_2_4_native(self.qkv_qweight, x, self.qkv_meta, self.qkv_scale, indices, base_weight=self.qkv_weight)

@@ -14,8 +14,8 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_st
     [B, width]).  Its new tokens are the last of them and stand in rows query_starts[b] .. query_starts[b + 1] of query
     (int32 [B + 1]; None: one new token per sequence).  A new token at position p sees the positions up to p (causal; all of
     the sequence otherwise), the last `window` of them where a window is given; a row that sees nothing is zero.  heads is a
-    multiple of the cache's heads.  Rows of out that belong to no sequence are left as they are; a negative page counts as
-    masked.  scale: 1 / sqrt(head_size) by default.
+    multiple of the cache's heads.  Rows of a given out that belong to no sequence are left as they are, those of a new one are
+    zero; a negative page counts as masked.  scale: 1 / sqrt(head_size) by default.
 
     What lies in the cache at or beyond a sequence's length, or before the window of all its new tokens, is never used.  Keys and
     values of the other tokens are finite numbers: a NaN or an infinity among them may reach every new token of its sequence,
