@@ -194,3 +194,34 @@ def test_a_missing_binding_fails_loudly(monkeypatch):
 def test_a_window_that_leaves_32_bits_is_refused():
     """Positions run from -num_tokens to the table's width, and a window is subtracted from them."""
     assert _attention(table_width=1 << 25, page_size=63, num_tokens=1 << 29, window=5) == 1
+
+
+def test_what_ctypes_binds_does_without_the_extension_module():
+    """It is built for one Python and one torch: the package imports without it, and only the operators that it binds say that it
+    is missing."""
+    import subprocess
+    import sys
+
+    code = """
+import sys
+sys.modules["triteia_b200._binding"] = None
+import torch
+from triteia_b200 import capi, nn, ops, triteia_cuda
+qweight, q, s, meta = ops.gen_sparse_quant4_NT(256, 128, device="cpu")
+try:
+    ops.matmul_4bit_2_4(q, torch.randn(4, 128).half(), meta, s)
+except RuntimeError as e:
+    assert "CUDA" in str(e)
+x, slots = torch.zeros(3, 2, 64).half(), torch.zeros(3, dtype=torch.int64)
+for call in (lambda: ops.cache_write(x, x, x, x, slots), lambda: ops.cache_read(x, x, slots), lambda: ops.paged_attention(x, x, x, slots, slots),
+             lambda: capi.qk_norm_rotary_embedding(slots, x, x, 64, x, True)):
+    try:
+        call()
+    except ImportError as e:
+        assert "triteia_b200.build" in str(e)
+    else:
+        raise AssertionError("no error")
+print("fine")
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert res.returncode == 0 and "fine" in res.stdout, res.stderr

@@ -132,3 +132,16 @@ def load_binding():
         raise ImportError("triteia_b200/_binding.so is missing or does not load: run `python -m triteia_b200.build` "
                           "(there is no CPU or PyTorch fallback)") from e
     return _binding
+
+
+class _Binding:
+    """The extension module, loaded by the first call of one of its operators: it is built for one Python and one torch, and
+    what ctypes binds does without it."""
+
+    def __getattr__(self, name):
+        fn = getattr(load_binding(), name)
+        setattr(self, name, fn)
+        return fn
+
+
+binding = _Binding()

@@ -3,9 +3,7 @@ exponent byte b per token and head (value = code * 2^(b - 127); 127 for a head o
 means: paged_attention knows such heads by it).  A token's slot is page * page_size + place."""
 import torch
 
-from ..._lib import load_binding
-
-_binding = load_binding()
+from ..._lib import binding
 
 
 def new_cache(num_pages, page_size, kv_heads, head_size, dtype=torch.float16, quantised=False, device="cuda"):
@@ -20,10 +18,10 @@ def new_cache(num_pages, page_size, kv_heads, head_size, dtype=torch.float16, qu
 def cache_write(key, value, key_cache, value_cache, slots, key_exponents=None, value_exponents=None):
     """Stores key and value [T, kv_heads, head_size] (rows may be parts of a fused projection) at `slots` [T].  A slot outside
     the cache (-1: padding) is skipped; a slot comes at most once in a call."""
-    _binding.cache_write(key, value, key_cache, value_cache, slots, key_exponents, value_exponents)
+    binding.cache_write(key, value, key_cache, value_cache, slots, key_exponents, value_exponents)
 
 
 def cache_read(key_cache, value_cache, slots, key_exponents=None, value_exponents=None, dtype=None):
     """(key, value) [T, kv_heads, head_size] of the tokens at `slots` as numbers of `dtype` (the cache's own, or for an e4m3
     cache float16 or bfloat16); zeros for a slot outside the cache."""
-    return _binding.cache_read(key_cache, value_cache, slots, key_exponents, value_exponents, dtype)
+    return binding.cache_read(key_cache, value_cache, slots, key_exponents, value_exponents, dtype)

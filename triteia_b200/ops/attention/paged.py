@@ -1,9 +1,7 @@
 """Attention of new tokens over a paged cache: single tokens, chunks of prompts, whole prompts and mixtures of them in one
 call.  Stands for the decode and extend programs of the reference (triteia/triton/decode_attention.py:30-214,
 extend_attention.py:39-170) and for its one-sequence wrapper (triteia/python/ops/attention/sdpa.py:25)."""
-from ..._lib import load_binding
-
-_binding = load_binding()
+from ..._lib import binding
 
 
 def paged_attention(query, key_cache, value_cache, page_table, lengths, query_starts=None, scale=None, causal=True, window=None,
@@ -20,5 +18,5 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_st
     What lies in the cache at or beyond a sequence's length, or before the window of all its new tokens, is never used.  Keys and
     values of the other tokens are finite numbers: a NaN or an infinity among them may reach every new token of its sequence,
     also those that do not see it."""
-    return _binding.paged_attention(query, key_cache, value_cache, page_table, lengths, query_starts, scale, causal, window, key_exponents,
-                                    value_exponents, out)
+    return binding.paged_attention(query, key_cache, value_cache, page_table, lengths, query_starts, scale, causal, window, key_exponents,
+                                   value_exponents, out)

@@ -9,9 +9,7 @@ pointers, the launch goes to torch's current stream of the tensors' device.
 import torch
 
 from . import _lib
-from ._lib import lib, ptr, stream_of, dev_of
-
-_binding = _lib.load_binding()
+from ._lib import binding, lib, ptr, stream_of, dev_of
 
 
 def _check_input(t, name):
@@ -189,4 +187,4 @@ def qk_norm_rotary_embedding(positions, query, key, head_size, cos_sin_cache, is
     eps=None: no norm, the weights and the rotation alone.  In place, or into query_out / key_out.  query [..., num_heads * head_size] and key [..., num_kv_heads * head_size] may be
     column ranges of a fused projection; cos_sin_cache [max_position, rot_dim] has query's dtype or float32.  A token whose
     position lies outside the cache is left alone."""
-    _binding.qk_norm_rotary(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight, key_weight, eps, query_out, key_out)
+    binding.qk_norm_rotary(positions, query, key, head_size, cos_sin_cache, is_neox, query_weight, key_weight, eps, query_out, key_out)
