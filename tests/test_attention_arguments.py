@@ -225,3 +225,24 @@ print("fine")
 """
     res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert res.returncode == 0 and "fine" in res.stdout, res.stderr
+
+
+def test_an_extension_module_for_another_torch_is_built_again(monkeypatch, tmp_path):
+    from triteia_b200 import build
+
+    assert build.binding_fits() and _lib.load_binding().built_for == build.binding_tag()
+    made = []
+
+    def compiled(cmd, **kw):
+        made.append(cmd)
+        return type("Result", (), dict(returncode=0, stdout="", stderr=""))()
+
+    monkeypatch.setattr(build.subprocess, "run", compiled)
+    build.build_binding()
+    assert not made                                    # it is there, newer than its sources, and fits
+    monkeypatch.setattr(build, "binding_tag", lambda: "triteia_b200 binding, torch 99.0, cpython-399")
+    build.build_binding()
+    assert len(made) == 1 and any("torch 99.0" in x for x in made[0])
+    with pytest.raises(ImportError, match="torch 99.0.*triteia_b200.build"):
+        _lib.load_binding()
+    assert not build.binding_fits(str(tmp_path / "none.so"))

@@ -126,6 +126,11 @@ def dtype_tag(dtype):
 
 def load_binding():
     """The extension module with the operators whose calls are short (csrc/binding.cpp); no fallback either."""
+    from .build import BINDING, binding_fits, binding_tag
+
+    if os.path.exists(BINDING) and not binding_fits():
+        raise ImportError(f"triteia_b200/_binding.so is not for this Python and torch ({binding_tag()}): run "
+                          "`python -m triteia_b200.build` (there is no CPU or PyTorch fallback)")
     try:
         from . import _binding
     except ImportError as e:

@@ -38,16 +38,32 @@ def needs_build():
     return any(os.path.getmtime(p) > t for p in sources() + [hdr])
 
 
+def binding_tag():
+    """What the extension module is built for; it holds this text.  Another Python or torch may refuse it, or crash in it."""
+    import torch
+
+    return f"triteia_b200 binding, torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def binding_fits(path=BINDING):
+    """Whether the extension module is there and built for this Python and torch."""
+    try:
+        with open(path, "rb") as f:
+            return binding_tag().encode() + b"\0" in f.read()
+    except FileNotFoundError:
+        return False
+
+
 def build_binding(force=False):
     """The extension module triteia_b200._binding; it finds libtriteia_b200.so next to itself."""
     hdr = os.path.join(PKG, "..", "include", "triteia_b200.h")
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(BINDING) >= os.path.getmtime(p) for p in (BINDING_SRC, hdr)):
+    if not force and binding_fits() and all(os.path.getmtime(BINDING) >= os.path.getmtime(p) for p in (BINDING_SRC, hdr)):
         return BINDING
     import torch
 
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
-    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DTRB_BINDING_TAG="{binding_tag()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
            + [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                                  os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
            + [BINDING_SRC, "-o", BINDING, f"-L{PKG}", "-ltriteia_b200", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",

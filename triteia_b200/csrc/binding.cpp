@@ -312,4 +312,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", TRB_BINDING_TAG) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
