@@ -298,6 +298,10 @@ int trb_paged_attention_clear(const void* query, const void* key_cache, const vo
  * device): pieces of the sequences that more than one CTA reads.  single: query_starts is NULL; e4m3: there are exponents. */
 size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
                                            int page_size, int table_width, int single, int e4m3, int dev);
+/* The same for a cache of these pages and strides: 0 for the calls that the tensor-memory kernel takes. */
+size_t trb_paged_attention_cache_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                                 int page_size, long long num_pages, int table_width, long long page_stride,
+                                                 long long token_stride, long long head_stride, int single, int e4m3, int dev);
 
 /* sums[r] = (accumulate ? sums[r] : 0) + sum over n of y[r, n]: fp32 per-row checksum of an fp16
  * matrix [rows, prob_m] (prob_m % 8 == 0, y 16-byte aligned), fixed summation order.  Used by the

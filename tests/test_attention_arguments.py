@@ -246,3 +246,14 @@ def test_an_extension_module_for_another_torch_is_built_again(monkeypatch, tmp_p
     with pytest.raises(ImportError, match="torch 99.0.*triteia_b200.build"):
         _lib.load_binding()
     assert not build.binding_fits(str(tmp_path / "none.so"))
+
+
+def test_workspace_only_for_the_calls_that_use_one():
+    def needs(tokens, seqs, page, width, head_stride=64, single=0):
+        return _lib.lib.trb_paged_attention_cache_workspace_bytes(tokens, seqs, 8, 2, 64, page, 100, width, page * 128, 128, head_stride, single, 0, 0)
+
+    assert needs(700, 3, 16, 200) == 0                 # tensor memory
+    for args in (dict(page=24), dict(page=16, head_stride=0)):
+        assert needs(700, 3, width=200, **args) == _lib.lib.trb_paged_attention_workspace_bytes(700, 3, 8, 2, 64, args["page"], 200, 0, 0, 0)
+    for tokens, single in ((3, 1), (3, 0)):
+        assert needs(tokens, 3, 16, 200, single=single) == _lib.lib.trb_paged_attention_workspace_bytes(tokens, 3, 8, 2, 64, 16, 200, single, 0, 0)

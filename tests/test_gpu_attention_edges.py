@@ -226,3 +226,14 @@ def test_delta_attention_of_a_padded_batch(cuda):
         outs.append(m(x[:rows], idx[:rows], pos[:rows], slots[:rows], cache, table, lengths, starts))
     assert torch.equal(outs[0][:T], outs[1])
     assert bool((outs[0][T:] == 0).all())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_prompt_takes_no_memory_but_its_output(cuda, e4m3):
+    b = Batch(88, [1500, 900], [700, 900], 8, 2, 128, 16, torch.float16, e4m3)
+    b.call()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = b.call()
+    assert torch.cuda.max_memory_allocated() - before == out.untyped_storage().nbytes()

@@ -50,6 +50,7 @@ SIGNATURES = {
     "trb_paged_attention": (_i, [_vp] * 9 + [_i] * 6 + [_ll, _ll, _i] + [_ll] * 10 + [_f] + [_i] * 3 + [_vp, _sz, _i, _vp]),
     "trb_paged_attention_clear": (_i, [_vp] * 9 + [_i] * 6 + [_ll, _ll, _i] + [_ll] * 10 + [_f] + [_i] * 3 + [_vp, _sz, _i, _vp, _i]),
     "trb_paged_attention_workspace_bytes": (_sz, [_i] * 10),
+    "trb_paged_attention_cache_workspace_bytes": (_sz, [_i] * 6 + [_ll, _i] + [_ll] * 3 + [_i] * 3),
     "trb_row_checksum": (_i, [_vp] * 2 + [_i] * 4 + [_vp]),
     "trb_stack_scratch_bytes": (_sz, [_i, _i]),
     "trb_stack_pass": (_i, [_i] + [_vp] * 5 + [_i, _vp] + [_vp] * 5 + [_i, _i, _vp, _i, _vp, _sz, _i, _vp]),

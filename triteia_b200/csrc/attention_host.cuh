@@ -18,6 +18,14 @@ static AttnKind attn_kind(long long tokens, int seqs, int group, bool single, bo
   return !single && tensor_fits ? kAttnTensor : kAttnRows;
 }
 
+// The stride of a dimension of one entry says nothing.
+static void attn_settle_strides(long long num_pages, int page_size, int kv_heads, int head_size, long long& page, long long& token,
+                                long long& head) {
+  if (kv_heads == 1) head = head_size;
+  if (page_size == 1) token = head_size;
+  if (num_pages == 1) page = head_size;
+}
+
 // Calls f with the configuration of the kernel for short calls.
 template <class T, class F>
 static auto attn_with_cfg(bool fp8, int head_size, bool rows, F f) {
@@ -38,7 +46,9 @@ static int launch_attn(const AttnArgs& a, int head_size, void* workspace, size_t
     else attn_clear_kernel<T, 64><<<ctas, 128, 0, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? TRB_OK : TRB_ERR_CUDA;
   }
-  const AttnKind kind = attn_kind(a.tokens, a.seqs, a.group, a.query_starts == nullptr, attn_tc_fits(a));
+  const bool single = a.query_starts == nullptr;
+  const AttnKind kind =
+      attn_kind(a.tokens, a.seqs, a.group, single, attn_tc_fits(single, a.page_size, a.num_pages, a.c_page, a.c_tok, a.c_head));
   if (kind == kAttnTensor) {
     if (head_size == 128) return fp8 ? launch_attn_tc<T, 128, true>(a, dev, st) : launch_attn_tc<T, 128, false>(a, dev, st);
     return fp8 ? launch_attn_tc<T, 64, true>(a, dev, st) : launch_attn_tc<T, 64, false>(a, dev, st);
@@ -55,13 +65,24 @@ extern "C" size_t trb_paged_attention_workspace_bytes(int num_tokens, int num_se
   if (num_tokens <= 0 || num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || page_size <= 0 || table_width < 0)
     return 0;
   const int group = num_heads / num_kv_heads;
-  // The tensor-memory kernel needs none, but whether it takes the call also depends on the cache's strides.
+  // The tensor-memory kernel needs none: the other bound says which calls it takes.
   const bool rows = attn_kind(num_tokens, num_seqs, group, single != 0, false) == kAttnRows;
   return attn_with_cfg<__half>(e4m3 != 0, head_size, rows, [&](auto cfg) -> size_t {
     using Cfg = decltype(cfg);
     const int ctas = attn_cut<Cfg>(num_tokens, num_seqs, group, num_kv_heads, single != 0, (long long)table_width * page_size, sm_count(dev)).ctas;
     return 2ull * ctas * Cfg::PIECE_FLOATS * 4;
   });
+}
+
+extern "C" size_t trb_paged_attention_cache_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                                            int page_size, long long num_pages, int table_width, long long page_stride,
+                                                            long long token_stride, long long head_stride, int single, int e4m3, int dev) {
+  using namespace trb;
+  if (num_tokens <= 0 || num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || page_size <= 0) return 0;
+  attn_settle_strides(num_pages, page_size, num_kv_heads, head_size, page_stride, token_stride, head_stride);
+  const bool fits = attn_tc_fits(single != 0, page_size, num_pages, page_stride, token_stride, head_stride);
+  if (attn_kind(num_tokens, num_seqs, num_heads / num_kv_heads, single != 0, fits) == kAttnTensor) return 0;
+  return trb_paged_attention_workspace_bytes(num_tokens, num_seqs, num_heads, num_kv_heads, head_size, page_size, table_width, single, e4m3, dev);
 }
 
 extern "C" int trb_paged_attention_clear(const void* query, const void* key_cache, const void* value_cache,
@@ -81,10 +102,7 @@ extern "C" int trb_paged_attention_clear(const void* query, const void* key_cach
       num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || table_width < 0 || (!page_table && table_width > 0 && num_seqs > 0) || window < 0)
     return TRB_ERR_BAD_ARG;
   if (!query_starts && (num_tokens != num_seqs || clear)) return TRB_ERR_BAD_ARG;
-  // The stride of a dimension of one entry says nothing.
-  if (num_kv_heads == 1) head_stride = head_size;
-  if (page_size == 1) token_stride = head_size;
-  if (num_pages == 1) page_stride = head_size;
+  attn_settle_strides(num_pages, page_size, num_kv_heads, head_size, page_stride, token_stride, head_stride);
   if (num_tokens == 1) query_token_stride = out_token_stride = 0;
   if (num_heads == 1) query_head_stride = out_head_stride = 0;
   if (num_heads % num_kv_heads != 0 || (window > 0 && !causal)) return TRB_ERR_PROB_SHAPE;

@@ -873,12 +873,11 @@ static int attn_tc_box(int page_size) {
 }
 
 // Whether the tensor-memory kernel takes the call: pages that hold whole groups of 16 tokens, strides that TMA takes.
-static bool attn_tc_fits(const AttnArgs& a) {
-  if (a.query_starts == nullptr) return false;
-  if (attn_tc_box(a.page_size) < 16 || a.num_pages <= 0 || a.num_pages >= 0x7fffffffLL) return false;
-  if (a.c_head <= 0 || a.c_tok <= 0 || a.c_page <= 0) return false;
+static bool attn_tc_fits(bool single, int page_size, long long num_pages, long long page_stride, long long token_stride, long long head_stride) {
+  if (single || attn_tc_box(page_size) < 16 || num_pages <= 0 || num_pages >= 0x7fffffffLL) return false;
+  if (head_stride <= 0 || token_stride <= 0 || page_stride <= 0) return false;
   const long long most = 1LL << 38;                   // strides of a tensor map: below 2^40 bytes
-  return a.c_head < most && a.c_tok < most && a.c_page < most;
+  return head_stride < most && token_stride < most && page_stride < most;
 }
 
 template <class T, int D, bool FP8>

@@ -236,7 +236,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int width = small(table.size(1), "page table's width");
   // A buffer of each call's own: calls on different streams, and graphs that are replayed side by side, share nothing.
   at::Tensor workspace;
-  const size_t bytes = trb_paged_attention_workspace_bytes(T, B, heads, c.heads, size, c.page_size, width, starts == nullptr, c.key_exp != nullptr, dev);
+  const size_t bytes = trb_paged_attention_cache_workspace_bytes(T, B, heads, c.heads, size, c.page_size, c.pages, width, c.page, c.token,
+                                                                 c.head, starts == nullptr, c.key_exp != nullptr, dev);
   if (bytes > 0) workspace = fresh_tensor({(int64_t)bytes}, at::kByte, device);
   // Rows of a new tensor that belong to no sequence are zeros, not what lay in the memory before.
   const int status = trb_paged_attention_clear(
