@@ -257,3 +257,13 @@ def test_workspace_only_for_the_calls_that_use_one():
         assert needs(700, 3, width=200, **args) == _lib.lib.trb_paged_attention_workspace_bytes(700, 3, 8, 2, 64, args["page"], 200, 0, 0, 0)
     for tokens, single in ((3, 1), (3, 0)):
         assert needs(tokens, 3, 16, 200, single=single) == _lib.lib.trb_paged_attention_workspace_bytes(tokens, 3, 8, 2, 64, 16, 200, single, 0, 0)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 1e300, -3e38])
+def test_a_scale_that_is_no_finite_number_is_refused(scale):
+    kc, vc, _, _ = ops.new_cache(PAGES, P, H, D, device="cpu")
+    x = torch.zeros(3, H, D, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="scale"):
+        ops.paged_attention(x, kc, vc, torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32), scale=scale)
+    if abs(scale) < 1e39 or scale != scale or abs(scale) == float("inf"):
+        assert _attention(scale=scale) == 3

@@ -113,6 +113,8 @@ extern "C" int trb_paged_attention_clear(const void* query, const void* key_cach
   // Positions are 32-bit numbers; the largest unit starts below length + 64.
   const long long most = (long long)table_width * page_size;
   if (most > 0x7fff0000LL || (long long)num_tokens * (num_heads / num_kv_heads) > 0x7fff0000LL) return TRB_ERR_PROB_SHAPE;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(fabsf(scale_log2) <= 3.402823466e38f)) return TRB_ERR_BAD_ARG;
   // A window as wide as the table hides nothing.  A narrower one is subtracted from positions down to -num_tokens (more new tokens
   // than the cache has).
   if (window >= most) window = 0;
@@ -124,7 +126,7 @@ extern "C" int trb_paged_attention_clear(const void* query, const void* key_cach
   const AttnArgs a{query, key_cache, value_cache, (const uint8_t*)key_exponents, (const uint8_t*)value_exponents,
                    (const int*)page_table, (const int*)lengths, (const int*)query_starts, out, query_token_stride, query_head_stride,
                    out_token_stride, out_head_stride, page_stride, token_stride, head_stride, exp_page_stride, exp_token_stride,
-                   exp_head_stride, table_stride, num_pages, scale * 1.4426950408889634f, num_tokens, num_seqs, num_kv_heads,
+                   exp_head_stride, table_stride, num_pages, scale_log2, num_tokens, num_seqs, num_kv_heads,
                    num_heads / num_kv_heads, page_size, table_width,
                    (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1, causal, window, clear != 0};
   if (dtype == TRB_F16) return launch_attn<__half>(a, head_size, workspace, workspace_bytes, dev, (cudaStream_t)stream);

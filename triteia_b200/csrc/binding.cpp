@@ -12,6 +12,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -221,6 +222,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (starts) check_vector(*starts, "query_starts", at::kInt, (int64_t)B + 1, device);
   else if (T != B) refuse("%d tokens for %d sequences: query_starts is needed", T, B);
   const double scale = args[6] == Py_None ? 1.0 / sqrt((double)size) : real(args[6]);
+  if (size > 0 && !(fabs(scale) <= 2e38)) refuse("scale must be a finite number that 32 bits hold");
   const bool causal = truth(args[7]);
   const long long window = args[8] == Py_None ? 0 : integer(args[8]);
   if (args[8] != Py_None && (window <= 0 || !causal)) refuse("a window is a positive number of tokens and needs causal=True");
