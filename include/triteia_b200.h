@@ -273,7 +273,8 @@ int trb_cache_read(const void* key_cache, const void* value_cache, const void* k
  * outside every sequence are not written.  What lies in the cache at or beyond a sequence's length, or before the window of
  * all its new tokens, is never used; keys and values of the other tokens are finite numbers (a NaN or an infinity among them
  * may reach every new token of its sequence).
- * scale is finite, also times log2(e).  query and out [T, num_heads, head_size] of `dtype` with strides that are multiples of 8; head_size 64 or 128.
+ * scale is finite, also times log2(e).  query and out [T, num_heads, head_size] of `dtype` with strides that are
+ * multiples of 8; head_size 64 or 128.
  * Stands for the programs of triteia/triton/decode_attention.py:30-214 and extend_attention.py:39-170. */
 int trb_paged_attention(const void* query, const void* key_cache, const void* value_cache, const void* key_exponents,
                         const void* value_exponents, const void* page_table, const void* lengths, const void* query_starts,

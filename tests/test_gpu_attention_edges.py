@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from test_gpu_attention import LONG_SHORT, SHORT, Batch, gen, normal, plain_attention, tolerance
-from triteia_b200 import ops
+from triteia_b200 import capi, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -237,3 +237,23 @@ def test_a_prompt_takes_no_memory_but_its_output(cuda, e4m3):
     torch.cuda.reset_peak_memory_stats()
     out = b.call()
     assert torch.cuda.max_memory_allocated() - before == out.untyped_storage().nbytes()
+
+
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("rot", [16, 24, 20, 0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rotation_alone_passes_on_what_it_does_not_turn(cuda, neox, rot, dtype):
+    """Sizes behind rot_dim come out as they are, infinities and NaN too, and reach no other size."""
+    g = gen(90)
+    q = normal(g, 9, 4 * 64, dtype=dtype)
+    angle = torch.rand(50, rot // 2, generator=g, device="cuda") * 6.28
+    table = torch.cat([angle.cos(), angle.sin()], 1)
+    clean = q.clone()
+    x = q.view(9, 4, 64)
+    x[1, 0, rot], x[2, 1, rot + 3], x[3, 2, 63], x[4, 3, rot + 6] = float("inf"), float("-inf"), float("nan"), float("inf")
+    spoilt, pos = q.clone(), torch.arange(9, device="cuda")
+    for t in (q, clean):
+        capi.qk_norm_rotary_embedding(pos, t, None, 64, table, neox, eps=None)
+    tail = torch.cat([t.view(9, 4, 64)[..., rot:].flatten().nan_to_num(7, 8, 9) for t in (q, spoilt)])
+    assert torch.equal(tail[:tail.numel() // 2], tail[tail.numel() // 2:])
+    assert torch.equal(q.view(9, 4, 64)[..., :rot], clean.view(9, 4, 64)[..., :rot])

@@ -79,8 +79,10 @@ struct QkNormArgs {
 constexpr int kQkThreads = 128;
 constexpr int kQkHeads = 5;           // heads of a group, all loaded together
 // NeoX and GPT-J; "Any": rot_dim / 2 is no multiple of 8 (4), or the table or the weights are not 16-byte aligned, so that
-// cosines, sines and weights come one by one (and a NeoX partner through shared memory).
-enum RotMode { kNeox, kNeoxAny, kPairs, kPairsAny };
+// cosines, sines and weights come one by one (and a NeoX partner through shared memory).  "Part": without a norm, sizes that are
+// not turned pass as they are, so that 0 * infinity must not reach them (with a norm an infinity leaves nothing of its head);
+// a form of its own because the test costs the others 2 % (8191 x 80 heads 57 -> 58 us).
+enum RotMode { kNeox, kNeoxPart, kNeoxAny, kPairs, kPairsPart, kPairsAny };
 
 __device__ __forceinline__ float table_value(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float table_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -102,7 +104,8 @@ __device__ __forceinline__ void table_values(const TC* p, float* v) {
 template <class T, class TC, int G, int MODE>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNormArgs a) {
   constexpr int GROUPS = kQkThreads / G;
-  constexpr bool PAIRS = MODE == kPairs || MODE == kPairsAny;
+  constexpr bool PAIRS = MODE == kPairs || MODE == kPairsPart || MODE == kPairsAny;
+  constexpr bool NEOX = MODE == kNeox || MODE == kNeoxPart, PART = MODE != kNeox && MODE != kPairs;
   __shared__ uint4 swap[MODE == kNeoxAny ? GROUPS : 1][MODE == kNeoxAny ? G : 1];
   const long long t = blockIdx.x;
   const int li = threadIdx.x % G, grp = threadIdx.x / G;
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
   float own[8], other[8];
   const bool there = pos >= 0 && pos < a.max_position;        // not: a padding token
   const TC* row = static_cast<const TC*>(a.table) + (there ? pos : 0) * a.rot_dim;
-  if constexpr (MODE == kNeox || MODE == kPairs) {
+  if constexpr (NEOX || (PAIRS && MODE != kPairsAny)) {
     // A lane's eight elements turn together or not at all.
     const bool turn = there && d0 < a.rot_dim;
     const int i = !turn ? 0 : PAIRS ? d0 >> 1 : d0 < half ? d0 : d0 - half;
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
     if (h >= heads) break;
     // The partners' inputs come over as they are, two to a word; their factor of the norm is this head's too.
     uint4 them = raw[u];
-    if constexpr (MODE == kNeox) {
+    if constexpr (NEOX) {
       const int hl = half >> 3;
       const int src = li < hl ? li + hl : li < 2 * hl ? li - hl : li;
       them.x = __shfl_sync(lanes, raw[u].x, src, G);
@@ -203,7 +206,8 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
     const float r = a.eps < 0.f ? 1.f : rsqrtf(sum * inv_size + a.eps);      // eps < 0: the rotation alone
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 p = PAIRS ? make_float2(x[e].y, x[e].x) : two_of(theirs[e], T());
+      float2 p = PAIRS ? make_float2(x[e].y, x[e].x) : two_of(theirs[e], T());
+      if (PART && d0 + 2 * e >= a.rot_dim) p = make_float2(0.f, 0.f);
       const float2 y = fma2(x[e], make_float2(own[2 * e], own[2 * e + 1]), mul2(p, make_float2(other[2 * e], other[2 * e + 1])));
       mine[e] = word_of(mul2(y, make_float2(r, r)), T());
     }
@@ -214,8 +218,10 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rotary_kernel(const QkNorm
 template <class T, class TC, int G>
 static void launch_qk_norm(const QkNormArgs& a, int mode, dim3 grid, cudaStream_t st) {
   if (mode == kNeox) qk_norm_rotary_kernel<T, TC, G, kNeox><<<grid, kQkThreads, 0, st>>>(a);
+  else if (mode == kNeoxPart) qk_norm_rotary_kernel<T, TC, G, kNeoxPart><<<grid, kQkThreads, 0, st>>>(a);
   else if (mode == kNeoxAny) qk_norm_rotary_kernel<T, TC, G, kNeoxAny><<<grid, kQkThreads, 0, st>>>(a);
   else if (mode == kPairs) qk_norm_rotary_kernel<T, TC, G, kPairs><<<grid, kQkThreads, 0, st>>>(a);
+  else if (mode == kPairsPart) qk_norm_rotary_kernel<T, TC, G, kPairsPart><<<grid, kQkThreads, 0, st>>>(a);
   else qk_norm_rotary_kernel<T, TC, G, kPairsAny><<<grid, kQkThreads, 0, st>>>(a);
 }
 
@@ -231,7 +237,9 @@ static void launch_qk_norm(const QkNormArgs& a, int num_tokens, bool is_neox, in
   y = y < least ? least : y > most ? most : y;
   const dim3 grid(num_tokens, y, a.num_kv_heads > 0 ? 2 : 1);
   const bool aligned = (((uintptr_t)a.table | (uintptr_t)a.query_weight | (uintptr_t)a.key_weight) & 15) == 0;
-  const int mode = is_neox ? (aligned && a.rot_dim % 16 == 0 ? kNeox : kNeoxAny) : (aligned && a.rot_dim % 8 == 0 ? kPairs : kPairsAny);
+  const bool part = a.eps < 0.f && a.rot_dim < a.head_size;
+  const int mode = is_neox ? (!aligned || a.rot_dim % 16 != 0 ? kNeoxAny : part ? kNeoxPart : kNeox)
+                           : (!aligned || a.rot_dim % 8 != 0 ? kPairsAny : part ? kPairsPart : kPairs);
   switch (g) {
     case 1: launch_qk_norm<T, TC, 1>(a, mode, grid, st); break;
     case 2: launch_qk_norm<T, TC, 2>(a, mode, grid, st); break;
