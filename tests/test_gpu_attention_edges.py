@@ -257,3 +257,14 @@ def test_rotation_alone_passes_on_what_it_does_not_turn(cuda, neox, rot, dtype):
     tail = torch.cat([t.view(9, 4, 64)[..., rot:].flatten().nan_to_num(7, 8, 9) for t in (q, spoilt)])
     assert torch.equal(tail[:tail.numel() // 2], tail[tail.numel() // 2:])
     assert torch.equal(q.view(9, 4, 64)[..., :rot], clean.view(9, 4, 64)[..., :rot])
+
+
+@pytest.mark.parametrize("new,page", KERNELS)
+def test_huge_keys_and_tiny_queries(cuda, new, page):
+    """Keys of about 2^118 and queries of about 2^-118: ordinary scores."""
+    b = Batch(91, [300, 700], [new, new], 8, 2, 128, page, torch.bfloat16, True)
+    for i, n in enumerate(b.lengths):
+        page_, place = places(b, i, range(n))
+        b.ke[page_, place] += 118
+    b.q = (b.q.float() * 2.0 ** -118).bfloat16()
+    check(b, b.call())

@@ -458,10 +458,11 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
       const float2 kf = *reinterpret_cast<const float2*>(exps + n * 8 + 2 * quad);
       const float2 ev = *reinterpret_cast<const float2*>(exps + Cfg::UNIT + n * 8 + 2 * quad);
       iv[n] = *reinterpret_cast<const float2*>(exps + 2 * Cfg::UNIT + n * 8 + 2 * quad);
-      s[n][0] = fmaf(s[n][0] * kf.x, c_row[0], ev.x);
-      s[n][1] = fmaf(s[n][1] * kf.y, c_row[0], ev.y);
-      s[n][2] = fmaf(s[n][2] * kf.x, c_row[1], ev.x);
-      s[n][3] = fmaf(s[n][3] * kf.y, c_row[1], ev.y);
+      // The row's and the key's factor first: they may be far from 1 on opposite sides.
+      s[n][0] = fmaf(s[n][0], kf.x * c_row[0], ev.x);
+      s[n][1] = fmaf(s[n][1], kf.y * c_row[0], ev.y);
+      s[n][2] = fmaf(s[n][2], kf.x * c_row[1], ev.x);
+      s[n][3] = fmaf(s[n][3], kf.y * c_row[1], ev.y);
     }
   } else {
 #pragma unroll
