@@ -371,28 +371,23 @@ __device__ __forceinline__ int attn_row_shift(float top) {
 // while its weight times 2^90 enters the sum as ever: 2^(90 + 8) a token, far from the end of 32 bits for 2^17 tokens and more.
 constexpr int kZeroValueExp = -90;
 
-// Whether all of a head's `chunks` 16-byte pieces of codes are zeros, of either sign.
-template <int CHUNKS, class Load>
-__device__ __forceinline__ bool attn_zero_codes(Load load) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const uint4 w = load(c);
-    any |= w.x | w.y | w.z | w.w;
-  }
-  return (any & 0x7f7f7f7fu) == 0;
-}
+// Whether 16 codes are zeros, of either sign.
+__device__ __forceinline__ bool attn_zero_codes(uint4 w) { return ((w.x | w.y | w.z | w.w) & 0x7f7f7f7fu) == 0; }
 
 // Gives the tokens of `maybe` (byte 127) whose value codes in shared memory are zeros their exponent; a warp for itself.  Not
 // inlined: the loop that hardly ever calls it has to stay in the instruction cache.
 template <class Cfg>
 __device__ __noinline__ void attn_zero_values(unsigned long long maybe, uint32_t vbase, float* exps, int lane) {
 #pragma unroll 1
-  for (int r = lane; r < 16 * Cfg::NT; r += 32)
-    if ((maybe >> r) & 1 && attn_zero_codes<Cfg::CHUNKS>([&](int c) { return lds128(vbase + attn_swizzle<Cfg::ROWB>(r, c)); })) {
+  for (int r = lane; r < 16 * Cfg::NT; r += 32) {
+    bool zeros = (maybe >> r) & 1;
+#pragma unroll 1
+    for (int c = 0; zeros && c < Cfg::CHUNKS; ++c) zeros = attn_zero_codes(lds128(vbase + attn_swizzle<Cfg::ROWB>(r, c)));      // real values: once
+    if (zeros) {
       exps[Cfg::UNIT + r] = (float)kZeroValueExp;
       exps[2 * Cfg::UNIT + r] = __uint_as_float((uint32_t)(127 - kZeroValueExp) << 23);
     }
+  }
   __syncwarp();
 }
 
