@@ -19,9 +19,10 @@
 // borders.  An item inside a run is finished there; of one that a border cuts, the pieces' states (maximum, sum, weighted
 // values) go to the caller's workspace, and a second launch joins them in the order of the tokens: no counters, nothing to
 // clear, a fixed order of the sums.
-// Measured: 64 sequences of 100 to 8000 tokens, 32 heads over 8 of 128, bf16: 161 us, 6.0 TB/s of the 6.55 that a copy reaches;
-// three of 90000 to 131072 tokens, e4m3: 132 us, 5.1 TB/s -- there the conversions make the loop longer than the instruction
-// cache takes well (two of three stalled cycles wait for instructions).  Clusters for all calls (one launch, no workspace)
+// Measured in a graph (and as calls in a row through Python): 64 sequences of 100 to 8000 tokens, 32 heads over 8 of 128, bf16:
+// 163 us (172), 6.0 TB/s of the 6.55 that a copy reaches; three of 90000 to 131072 tokens, e4m3: 135 to 140 us (148), 4.8 to 5.0
+// TB/s -- there the conversions make the loop longer than the instruction cache takes well (two of three stalled cycles wait for
+// instructions).  Clusters for all calls (one launch, no workspace)
 // left half of the SMs idle with twelve CTAs each and unequal sequences unequal: 184 and 197 us.
 // Loads are 16-byte cp.async with a row address per token (any page size and strides); a token outside the visible range
 // or on a page outside the cache is filled with zeros and masked.
@@ -353,7 +354,8 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 }
 
 // The e4m3 form computes in fp16 whatever T is: a code is exact in fp16, and a bf16 query row, scaled by a power of two
-// to a largest magnitude of 2^9 .. 2^10, keeps all its bits down to 2^-25 of that.  Weights are fp16 there (11 bits).
+// to a largest magnitude of 2^9 .. 2^10, keeps all its bits down to 2^-25 of that; what is smaller is off by 2^-34 of the largest
+// (half of fp16's last step), as a rule far less than the 32-bit sum of the score rounds off.  Weights are fp16 there (11 bits).
 template <class T, bool FP8>
 struct AttnMma { using type = T; };
 template <class T>
@@ -520,7 +522,9 @@ __device__ __forceinline__ void attn_block(AttnState<Cfg::D>& st, const uint32_t
       if constexpr (Cfg::FP8) st.l[e >> 1] = fmaf(p, e & 1 ? iv[n].y : iv[n].x, st.l[e >> 1]);
       else st.l[e >> 1] += p;
     }
-  // ---- values: the weights are rounded to the MMA type (half a step, of random sign), the sum above is not.
+  // ---- values: the weights are rounded to the MMA type (half a step, of random sign), the sum above is not.  That adds about as
+  // much to the output's error as its own rounding (bf16 2.1e-3 of it in all against 1.7e-3, fp16 2.5e-4 against 2.0e-4); weights
+  // in two parts would keep their bits for half as many MMAs again.
   const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = lane >> 4;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {

@@ -11,6 +11,10 @@ namespace trb {
 // us, 24 of each of 32 after 2000: 64 and 118, 700 after 800 next to 127 single ones after 1000: 150 and 228; 6 of each of 200
 // after 900: 217 and 221, of size 64 e4m3 122 and 112, its worst.  Below 17 rows splitting the tokens wins (4 of each of 128 after
 // 1000: 134 and 103).
+// The host knows the average alone.  A chunk beside so many single or empty sequences that the average stays below 17 rows walks
+// its keys 16 rows at a time: in a graph, against the chunk and the rest as two calls, 512 of 1512 next to 63 single ones, 32 heads
+// over 32, bf16: 228 us against 193; 700 of 1500 next to 240 single ones, 32 over 8: 276 against 197; 900 of 12000 next to 63
+// single ones, 32 over 32: 1425 against 367, next to 63 empty ones 1204 against 200.  Two calls are the better way there.
 enum AttnKind { kAttnSplit, kAttnRows, kAttnTensor };
 static AttnKind attn_kind(long long tokens, int seqs, int group, bool single, bool tensor_fits) {
   const long long rows = single ? (long long)group * seqs : tokens * group;

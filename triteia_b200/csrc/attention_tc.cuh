@@ -1,5 +1,6 @@
-// Attention of new tokens over a paged cache on the fifth-generation tensor cores: the calls that the matrix products
-// bound (prompts, long chunks), with a cache of the inputs' type.  Definition and masks as in attention.cuh.
+// Attention of new tokens over a paged cache on the fifth-generation tensor cores: prompts, chunks and other calls of more than
+// 16 rows for an average sequence, over caches of the inputs' type or e4m3 whose pages hold whole groups of 16 tokens.  Definition
+// and masks as in attention.cuh.
 //
 // A CTA owns 256 rows (token, query head of the group) of one sequence and key head, as two tiles of 128, and walks the
 // visible keys in tiles of 128.  While the tensor cores work on one tile, the other one's softmax runs:
@@ -9,27 +10,32 @@
 //   values   O += P V    A operand = the weights in tensor memory, B operand = V rows as they lie in memory (MN-major)
 // so scores and weights never touch shared memory.  O stays in tensor memory; it is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time (the weights are then at most 2^8 times what they would be, which fp32
-// sums and fp16 or bf16 weights hold), so almost never after the first tiles.
+// sums and fp16 or bf16 weights hold), so almost never after the first tiles.  Two row tiles in turn and the rare rescaling are
+// known from published work on attention for this generation of tensor cores; roles, barriers and the e4m3 path are this file's.
 //   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (TMEM lanes 32 * (warp % 4) ..)
 //   warp 8           issues the MMAs (an elected lane), owns the tensor memory
 //   warp 9           loads: one box per page and 64 sizes, a lane per page.  A page outside the cache, and boxes that no
 //                    row sees, become boxes past the end of the cache, which TMA fills with zeros.
-//   warps 10, 11     complete the third warpgroup, which hands registers to the other two
+//   warps 10, 11     complete the third warpgroup, which hands registers to the other two; e4m3: exponents and factors; rows of
+//                    the output that belong to no sequence, where they are to be zero
 // Order of the MMAs: S0(0) S1(0), then for every key tile O0 += P0 V, S0(next), O1 += P1 V, S1(next): S(next) of a tile may
 // overwrite its P because the pipe runs in order, and when S(next) is complete so is that tile's O.
 //
-// An e4m3 cache: the codes land in a ring of their own and four more warps (12-15) turn them into fp16 tiles, exactly; the
-// powers of two enter at the scores, as in attention.cuh: 2^(t_j - m) with t_j = log2 weight + e_j meets the code of v_j.
+// An e4m3 cache: the codes land in a ring of their own and four more warps (12-15) turn them into fp16 tiles, exactly: times
+// 2^(e_j - E), E the largest exponent among their 128 tokens, but no less than 2^-15, the last factor that leaves every code a
+// number of fp16.  What is left of the power enters per token, at the scores: the keys' as a factor, the values' as in
+// attention.cuh, where 2^(t_j - m) with t_j = log2 weight + e_j meets the code of v_j.  A head of zeros has no part in E.
 // Queries and weights are fp16 there whatever T is (queries scaled by a power of two per row).
 //
 // A call with few items over long keys gives each item to a cluster of 2, 4 or 8 CTAs, which walk a run of its key tiles each
 // and join their states over distributed shared memory; the rule and its figures stand at the launch.
 //
-// Measured (32 heads of 128): a prompt of 8192 tokens over 32 key heads, fp16, 516 us = 1.07 PFLOP/s (605 us in a loop, where
-// the power cap holds the clock at 1.64 GHz); five chunks of 20 to 700 tokens over 1020 to 6000, 8 key heads, bf16, 145 us; two
-// chunks over 8362 and 12000 e4m3 tokens 301 us.  A key tile takes a CTA about 3400 clocks, of which the MMAs need 2048 and the
-// exponentials as many (16 a clock); the rest is the way of one tile from its scores to the next ones.  Calls of one to a few
-// waves lose most to the last one.  Cutting them like the short calls (persistent CTAs, pieces joined) cost 8 us a piece and was
+// Measured (32 heads of 128): a prompt of 8192 tokens over 32 key heads, fp16, 515 us = 1.07 PFLOP/s (600 to 615 us in a loop,
+// where the power cap holds the clock at 1.64 GHz); five chunks of 20 to 700 tokens over 1020 to 6000, 8 key heads, bf16, 147 us in
+// a graph and 153 as calls in a row; two chunks over 8362 and 12000 e4m3 tokens 308 and 311.  A key tile takes a CTA about 3400
+// clocks, of which the MMAs need 2048 and the exponentials as many (16 a clock); the rest is the way of one tile from its scores to
+// the next ones.  The prompt's 228 key tiles an SM are 395 us of that at 1.965 GHz and 473 at 1.64; the rest of its time, entry and
+// exit of seven items an SM and the clock of a short run, is not told apart.  Calls of one to a few waves lose most to the last one.  Cutting them like the short calls (persistent CTAs, pieces joined) cost 8 us a piece and was
 // slower (152 -> 190 us); so were clusters of two where they do not all run at once (chunks 144 -> 152, e4m3 300 -> 307).
 // Moving a quarter or half of the exponentials to the multiply-add pipe changed the chunks by -2 and +1 %, the prompt by +1 and
 // +6 %.

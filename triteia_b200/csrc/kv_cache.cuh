@@ -11,8 +11,9 @@
 // Bytes bound both kernels.  A group of G lanes moves one head, 16 bytes of inputs a lane; the maximum of a head is
 // log2(G) shuffles, so a token is read once.  A CTA works on one token: its slot is split into page and place once, and each
 // group has the loads of up to five heads' keys or values in flight before the first is worked on.  8192 tokens x 40 heads of
-// 128, fp16 and e4m3: write 51 us (4.9 TB/s; its rounding and packing share the issue slots with the loads), read 41 us
-// (6.1 TB/s).
+// 128, fp16 and e4m3, in a graph: write 51 us (4.9 TB/s; its rounding and packing share the issue slots with the loads), read 41
+// us (6.1 TB/s).  Five is the number for 40 heads; with 8 key heads a group has two loads in flight behind that of the slot
+// (1500 tokens written and 4000 read, bf16: 3 and 5.5 us, 4.1 and 5.9 TB/s, most of it in L2).
 #pragma once
 
 #include <cuda_fp8.h>

@@ -7,8 +7,10 @@
 // A group of G = head_size / 8 lanes (rounded up to a power of two) holds one head, 8 elements = 16 bytes a lane: the sum of
 // squares is log2(G) shuffles, a NeoX partner's inputs come with four more.  A group has up to five heads of ONE token and
 // asks for all of them, for the position and then for its cosines and sines at once, so that a CTA waits for memory twice and
-// no more: with loops over the heads of a token (fewer and longer CTAs) 8191 x 80 heads took 80 to 90 us, now 57.5 (5.9 TB/s;
-// before the arithmetic went two numbers at a time 61 with five heads a group, 74 with four or eight).
+// no more: with loops over the heads of a token (fewer and longer CTAs) 8191 x 80 heads took 80 to 90 us, now 57 in a graph (5.9
+// TB/s; 63 as calls in a row; before the arithmetic went two numbers at a time 61 with five heads a group, 74 with four or eight).
+// Five is the number for 40 heads of queries and of keys.  Other numbers leave places empty, most of all few key heads, which have
+// CTAs of their own: 32 + 32 heads 50.6 us (5.3 TB/s), 64 + 8 66 (4.6), 32 + 8 39 (4.3).
 #pragma once
 
 #include "elementwise.cuh"

@@ -15,6 +15,10 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_st
     multiple of the cache's heads.  Rows of a given out that belong to no sequence are left as they are, those of a new one are
     zero; a negative page counts as masked.  scale: 1 / sqrt(head_size) by default.
 
+    head_size is 64 or 128, and heads begin on 16-byte boundaries (of an e4m3 cache too, where cache_write is content with 8).  Among
+    many single tokens or sequences without new ones, a chunk of hundreds is faster in a call of its own; a page table much wider
+    than the sequences are long costs small calls some microseconds.
+
     What lies in the cache at or beyond a sequence's length, or before the window of all its new tokens, is never used.  Keys and
     values of the other tokens are finite numbers: a NaN or an infinity among them may reach every new token of its sequence,
     also those that do not see it."""
