@@ -268,3 +268,47 @@ def test_huge_keys_and_tiny_queries(cuda, new, page):
         b.ke[page_, place] += 118
     b.q = (b.q.float() * 2.0 ** -118).bfloat16()
     check(b, b.call())
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv_heads", [([3000], [60], 8, 2), ([5000, 300, 900], [1, 1, 1], 8, 2), ([700], [1], 32, 32), ([9000, 20], [4, 2], 8, 2)],
+                         ids=["cluster", "line", "single", "few"])
+@pytest.mark.parametrize("ahead", [0, 30])
+def test_value_heads_of_zeros_where_several_ctas_share_a_sequence(cuda, lengths, new, heads, kv_heads, ahead):
+    """Long runs of zero heads, so that some of the pieces that are joined have nothing else."""
+    b = Batch(89, lengths, new, heads, kv_heads, 128, 16, torch.bfloat16, True)
+    b.q[..., 0] = 4
+    for i, n in enumerate(lengths):
+        page, place = places(b, i, range(n))
+        b.kc.view(torch.uint8)[page, place, :, 0] = 0
+        b.ve[page, place] = (b.ve[page, place].int() - 20).to(torch.uint8)
+        page, place = places(b, i, range(n // 8, n - n // 8))
+        b.kc[page, place, :, 0] = torch.tensor(ahead * 128 ** 0.5 / 4 / 16, device="cuda").to(torch.float8_e4m3fn)
+        b.vc.view(torch.uint8)[page, place] = 0
+        b.ve[page, place] = 127
+    for starts in (b.starts, None) if sum(new) == len(new) else (b.starts,):
+        b.starts = starts
+        check(b, b.call())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,new", [([300, 170], [40, 130]), ([4000, 70, 30], [2, 1, 1])], ids=["chunks", "few"])
+def test_a_replayed_graph_of_a_batch_that_shrinks(cuda, e4m3, lengths, new):
+    """A graph of fixed size: sequences that leave are padding in the next replay, and their rows are zeros."""
+    b = Batch(92, lengths, new, 8, 2, 128, 16, torch.float16, e4m3)
+    graph = torch.cuda.CUDAGraph()
+    b.call()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = b.call()
+    graph.replay()
+    b.check(out)
+    b.starts[-1] = b.starts[-2]
+    want = b.call()
+    graph.replay()
+    torch.cuda.synchronize()
+    live = sum(new[:-1])
+    assert torch.equal(out, want) and bool((out[live:] == 0).all())
+    b.starts.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())
